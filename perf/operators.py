@@ -1,0 +1,272 @@
+"""The attention-side layer operators of yolo_amd.utils.layer_utils as measured cases: `linear` (matrix product with bias,
+activation and residual), `qk_norm_rope` (per-head norms of queries and keys with the position rotation) and
+`cross_attention` (queries over the states of an encoder of another length).
+
+Sizes are those of the detectors here: feature maps of 13 x 13 to 76 x 76 cells (416 and 608 pixel inputs; 3549 cells are the
+three maps of a 416 pixel image end to end), 256 / 512 / 1024 channels, 255 = 3 * (5 + 80) head channels, 80 classes, batches of
+1 to 64 images.  `own` chooses between elementary torch operations in 32 bits (False) and the framework's kernels (True)."""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+# ---- cases -------------------------------------------------------------------------------------------------------------------
+def listed():
+    return [
+        # one query of one image through a projection layer: a step of a decoder that emits one token at a time; latency counts
+        dict(name="linear_step", op="linear", type="bf16", rows=1, k=1024, n=1024, bias=True, activation="silu", residual=False),
+        # the 255 channels of a detection head as rows of an odd width (510 bytes, no row but the first is aligned), a ragged row count
+        dict(name="linear_head_odd", op="linear", type="bf16", rows=1001, k=255, n=255, bias=True, activation="leaky", residual=True),
+        # all cells of the 52 x 52 map of 64 images, the output projection of a block with its residual: bandwidth counts
+        dict(name="linear_map", op="linear", type="bf16", rows=64 * 2704, k=256, n=512, bias=True, activation="gelu", residual=True),
+        # the widening layer of a block's feed-forward half on the 19 x 19 map of 64 images: the matrix cores count
+        dict(name="linear_mlp", op="linear", type="bf16", rows=64 * 361, k=1024, n=4096, bias=True, activation="gelu", residual=False),
+        # the parity type: 26 x 26 map of 8 images
+        dict(name="linear_f32", op="linear", type="f32", rows=8 * 676, k=512, n=512, bias=True, activation=None, residual=True),
+        # the query of one step, the keys were normalised when the encoder ran
+        dict(name="qk_step", op="qk", type="bf16", batch=1, lq=1, lk=0, hq=8, hk=8, d=64, axes=1, interleaved=False, start=811),
+        # queries of the 26 x 26 map and keys of the 52 x 52 map of 32 images, (row, column) positions
+        dict(name="qk_maps", op="qk", type="bf16", batch=32, lq=676, lk=2704, hq=8, hk=8, d=64, axes=2, interleaved=False, start=0),
+        # the parity type, shared key heads, pairs side by side, far positions
+        dict(name="qk_f32", op="qk", type="f32", batch=3, lq=361, lk=1444, hq=8, hk=2, d=128, axes=1, interleaved=True, start=100003),
+        # one query of one image over all cells of its three maps, four query heads to a key head
+        dict(name="xattn_step", op="xattn", type="bf16", batch=1, lq=1, lk=3549, hq=16, hk=4, d=64, mask="none"),
+        # a hundred object queries of each of 32 images over all cells of its maps, images of different sizes in one padded batch
+        dict(name="xattn_queries", op="xattn", type="bf16", batch=32, lq=100, lk=3549, hq=8, hk=8, d=64, mask="lens"),
+        # the parity type: every cell of the 26 x 26 map over 80 class prompts, some of them switched off
+        dict(name="xattn_text_f32", op="xattn", type="f32", batch=4, lq=676, lk=80, hq=8, hk=8, d=64, mask="keys"),
+        # every cell of the 52 x 52 map over every cell of the 76 x 76 map of the same 8 images at 608 pixels: the matrix cores count
+        dict(name="xattn_maps", op="xattn", type="bf16", batch=8, lq=2704, lk=5776, hq=8, hk=8, d=128, mask="none"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    op = rng.choice(("linear", "linear", "qk", "xattn", "xattn"))
+    kind = rng.choice(("bf16", "bf16", "f32"))
+    if op == "linear":
+        # rows from one query to a large batch's map; widths in whole 16-byte pieces or, one time in three, any
+        k, n = _log(rng, 16, 2048), _log(rng, 16, 4096)
+        if rng.random() < 2 / 3:
+            k, n = (k + 7) // 8 * 8, (n + 7) // 8 * 8
+        rows = _log(rng, 1, 180000)
+        limit = 9.0e10 if kind == "bf16" else 1.2e10
+        rows = max(1, min(rows, int(limit / (2.0 * k * n)), int(1.2e8 / max(k, n))))
+        return dict(op=op, type=kind, rows=rows, k=k, n=n, bias=rng.random() < 0.7,
+                    activation=rng.choice((None, "leaky", "relu", "gelu", "silu")), residual=rng.random() < 0.5)
+    d = rng.choice((32, 64, 64, 80, 96, 128, 128, 256))
+    hk = rng.choice((1, 2, 4, 8))
+    hq = hk * rng.choice((1, 1, 2, 4))
+    batch = _log(rng, 1, 64)
+    if op == "qk":
+        lq, lk = _log(rng, 1, 3549), rng.choice((0, _log(rng, 1, 3549)))
+        batch = max(1, min(batch, int(6.0e7 / ((lq * hq + lk * hk) * d))))
+        return dict(op=op, type=kind, batch=batch, lq=lq, lk=lk, hq=hq, hk=hk, d=d, axes=rng.choice((1, 2)),
+                    interleaved=rng.random() < 0.5, start=rng.choice((0, 0, _log(rng, 1, 1000000))))
+    lq, lk = _log(rng, 1, 3000), _log(rng, 1, 6000)
+    limit = 1.5e11 if kind == "bf16" else 1.2e10
+    batch = max(1, min(batch, int(limit / (4.0 * lq * lk * hq * d)), int(6.0e7 / ((lq * hq + 2 * lk * hk) * d))))
+    lq = max(1, min(lq, int(limit / (4.0 * batch * lk * hq * d))))
+    return dict(op=op, type=kind, batch=batch, lq=lq, lk=lk, hq=hq, hk=hk, d=d, mask=rng.choice(("none", "lens", "keys")))
+
+
+# ---- inputs ------------------------------------------------------------------------------------------------------------------
+def _positions(length, axes, start, device):
+    """[length] counting from `start`, or [length, 2] = (row, column) of the cells of a map about as wide as high."""
+    i = torch.arange(length, device=device, dtype=torch.int32)
+    if axes == 1:
+        return i + start
+    w = max(1, int(math.isqrt(length)))
+    return torch.stack((torch.div(i, w, rounding_mode="floor") + start, i % w + start), dim=-1).to(torch.int32)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(int(seed))
+    t = _TYPES[case["type"]]
+
+    def randn(*shape, scale=1.0):
+        return torch.randn(shape, generator=g, device="cuda", dtype=torch.float32).mul_(scale).to(t)
+
+    s = dict(case)
+    if case["op"] == "linear":
+        m, k, n = case["rows"], case["k"], case["n"]
+        s["x"] = randn(m, k)
+        s["w"] = randn(n, k, scale=k ** -0.5)
+        s["b"] = randn(n, scale=0.2) if case["bias"] else None
+        s["r"] = randn(m, n) if case["residual"] else None
+        return s
+    b, lq, lk, hq, hk, d = (case[x] for x in ("batch", "lq", "lk", "hq", "hk", "d"))
+    if case["op"] == "qk":
+        # queries and keys as one projection leaves them; norm weights near one
+        s["q"] = randn(b, lq, hq, d, scale=1.5)
+        s["k"] = randn(b, lk, hk, d, scale=0.7) if lk else None
+        s["qw"] = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(t)
+        s["kw"] = (1 + 0.1 * torch.randn(d, generator=g, device="cuda")).to(t) if lk else None
+        pairs = d // 2 // case["axes"]
+        f = 10000.0 ** (-torch.arange(pairs, device="cuda", dtype=torch.float64) / pairs)
+        s["f"] = f.repeat(case["axes"])                       # radians per position of every pair, the pairs of an axis together
+        s["qp"] = _positions(lq, case["axes"], case["start"], "cuda")
+        s["kp"] = _positions(lk, case["axes"], case["start"], "cuda") if lk else None
+        return s
+    # normalised queries and keys: scores of unit variance after the scale; keys and values are the two halves of one projection
+    s["q"] = randn(b, lq, hq, d)
+    kv = randn(b, lk, 2, hk, d)
+    s["kv"] = kv
+    s["lens"] = s["mask_keys"] = None
+    if case["mask"] == "lens":
+        s["lens"] = torch.randint(max(1, lk // 2), lk + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    elif case["mask"] == "keys":
+        s["mask_keys"] = torch.rand((b, lk), generator=g, device="cuda") < 0.8
+    return s
+
+
+# ---- one pass ----------------------------------------------------------------------------------------------------------------
+def _act(y, name):
+    if name is None:
+        return y
+    if name == "leaky":
+        return torch.where(y > 0, y, 0.1 * y)
+    if name == "relu":
+        return torch.where(y < 0, torch.zeros_like(y), y)
+    if name == "gelu":
+        return 0.5 * y * (1 + torch.erf(y * 0.5 ** 0.5))
+    return y / (1 + torch.exp(-y))
+
+
+def _norm_rope(x, w, f, p, interleaved, eps):
+    if x is None:
+        return None
+    h = x.float()
+    h = h * torch.rsqrt((h * h).mean(-1, keepdim=True) + eps) * w.float()
+    axes = 1 if p.dim() == 1 else p.shape[-1]
+    each = f.numel() // axes
+    pos = p.reshape(p.shape[0], axes, 1).expand(-1, -1, each).reshape(p.shape[0], -1).double()
+    a = (pos * f)[None, :, None, :]                           # far positions: the angle in 64 bits
+    c, s = torch.cos(a).float(), torch.sin(a).float()
+    if interleaved:
+        u, v = h[..., 0::2], h[..., 1::2]
+        y = torch.stack((u * c - v * s, u * s + v * c), dim=-1).flatten(-2)
+    else:
+        u, v = h.chunk(2, dim=-1)
+        y = torch.cat((u * c - v * s, u * s + v * c), dim=-1)
+    return y.to(x.dtype)
+
+
+def _attend(q, k, v, lens, keys):
+    b, lq, hq, d = q.shape
+    lk, hk = k.shape[1], k.shape[2]
+    g = hq // hk
+    qf = q.float().reshape(b, lq, hk, g, d).permute(0, 2, 3, 1, 4).reshape(b, hk, g * lq, d)
+    kf = k.float().permute(0, 2, 3, 1).contiguous()
+    vf = v.float().permute(0, 2, 1, 3).contiguous()
+    s = torch.matmul(qf, kf) * d ** -0.5
+    if lens is not None:
+        keys = torch.arange(lk, device=q.device)[None, :] < lens[:, None]
+    if keys is not None:
+        s = s.masked_fill(~keys[:, None, None, :], float("-inf"))
+    m = s.amax(-1, keepdim=True)
+    e = torch.exp(s - torch.where(m == float("-inf"), torch.zeros_like(m), m))
+    t = e.sum(-1, keepdim=True)
+    o = torch.matmul(e, vf) / torch.where(t == 0, torch.ones_like(t), t)
+    return o.reshape(b, hk, g, lq, d).permute(0, 3, 1, 2, 4).reshape(b, lq, hq, d).to(q.dtype)
+
+
+def run(s):
+    if own:
+        from yolo_amd.utils import layer_utils as L
+        if s["op"] == "linear":
+            return L.linear(s["x"], s["w"], s["b"], activation=s["activation"], residual=s["r"])
+        if s["op"] == "qk":
+            q, k = L.qk_norm_rope(s["q"], s["k"], s["qw"], s["kw"], frequencies=s["f"], q_positions=s["qp"], k_positions=s["kp"],
+                                  eps=1e-6, interleaved=s["interleaved"])
+            return (q,) if k is None else (q, k)
+        return L.cross_attention(s["q"], s["kv"][:, :, 0], s["kv"][:, :, 1], key_lens=s["lens"], key_mask=s["mask_keys"])
+    if s["op"] == "linear":
+        y = torch.matmul(s["x"].float(), s["w"].float().t())
+        if s["b"] is not None:
+            y = y + s["b"].float()
+        y = _act(y, s["activation"])
+        if s["r"] is not None:
+            y = y + s["r"].float()
+        return y.to(s["x"].dtype)
+    if s["op"] == "qk":
+        q = _norm_rope(s["q"], s["qw"], s["f"], s["qp"], s["interleaved"], 1e-6)
+        k = _norm_rope(s["k"], s["kw"], s["f"], s["kp"], s["interleaved"], 1e-6)
+        return (q,) if k is None else (q, k)
+    return _attend(s["q"], s["kv"][:, :, 0], s["kv"][:, :, 1], s["lens"], s["mask_keys"])
+
+
+def work(case):
+    z = 2 if case["type"] == "bf16" else 4
+    if case["op"] == "linear":
+        m, k, n = case["rows"], case["k"], case["n"]
+        return {"bytes": z * (m * k + n * k + m * n * (2 if case["residual"] else 1) + (n if case["bias"] else 0)), "flops": 2 * m * n * k}
+    b, lq, lk, hq, hk, d = (case[x] for x in ("batch", "lq", "lk", "hq", "hk", "d"))
+    if case["op"] == "qk":
+        e = b * (lq * hq + lk * hk) * d
+        return {"bytes": 2 * z * e + 4 * (lq + lk) * case["axes"] + 4 * d, "flops": 8 * e}
+    share = 0.75 if case["mask"] == "lens" else 1.0           # the mean length of a padded batch
+    return {"bytes": int(z * b * d * (2 * lq * hq + 2 * share * lk * hk)), "flops": int(4 * share * b * lq * lk * hq * d)}
+
+
+# ---- the definitions in 64 bits ------------------------------------------------------------------------------------------------
+def exact(case, seed):
+    s = prepare(case, seed)
+    if case["op"] == "linear":
+        y = torch.einsum("mk,nk->mn", s["x"].double(), s["w"].double())
+        if s["b"] is not None:
+            y += s["b"].double()
+        a = case["activation"]
+        if a == "leaky":
+            y = torch.maximum(y, y / 10)
+        elif a == "relu":
+            y = y.clamp(min=0)
+        elif a == "gelu":
+            y = y * torch.special.ndtr(y)
+        elif a == "silu":
+            y = y * torch.sigmoid(y)
+        return y if s["r"] is None else y + s["r"].double()
+    if case["op"] == "qk":
+        out = []
+        for x, w, p in ((s["q"], s["qw"], s["qp"]), (s["k"], s["kw"], s["kp"])):
+            if x is None:
+                continue
+            h = x.double()
+            h = h / torch.sqrt(h.square().sum(-1, keepdim=True) / case["d"] + 1e-6) * w.double()
+            pairs = case["d"] // 2
+            angle = torch.empty((x.shape[1], pairs), dtype=torch.float64, device=x.device)
+            for i in range(pairs):
+                axis = i * case["axes"] // pairs
+                angle[:, i] = (p[:, axis] if case["axes"] > 1 else p).double() * s["f"][i]
+            z = torch.polar(torch.ones_like(angle), angle)[None, :, None, :]
+            if case["interleaved"]:
+                y = torch.view_as_real(torch.view_as_complex(h.reshape(*h.shape[:-1], pairs, 2).contiguous()) * z).reshape(h.shape)
+            else:
+                c = torch.complex(h[..., :pairs].contiguous(), h[..., pairs:].contiguous()) * z
+                y = torch.cat((c.real, c.imag), -1)
+            out.append(y)
+        return tuple(out)
+    b, lq, hq, d = s["q"].shape
+    hk = case["hk"]
+    out = torch.zeros((b, lq, hq, d), dtype=torch.float64, device="cuda")
+    for i in range(b):
+        keep = torch.ones(case["lk"], dtype=torch.bool, device="cuda")
+        if s["lens"] is not None:
+            keep = torch.arange(case["lk"], device="cuda") < s["lens"][i]
+        elif s["mask_keys"] is not None:
+            keep = s["mask_keys"][i]
+        kk, vv = s["kv"][i, :, 0][keep].double(), s["kv"][i, :, 1][keep].double()
+        if kk.shape[0] == 0:
+            continue
+        for h in range(hq):
+            j = h * hk // hq
+            p = torch.softmax(s["q"][i, :, h].double() @ kk[:, j].t().contiguous() / math.sqrt(d), dim=-1)
+            out[i, :, h] = p @ vv[:, j].contiguous()
+    return out
