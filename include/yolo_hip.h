@@ -230,6 +230,46 @@ int yolo2_nms(const double* boxes, const float* probs, int B, int n, int C, floa
               int max_det, int32_t* out_counts, int32_t* out_cls, double* out_boxes, float* out_probs,
               int32_t* out_flat, int32_t* out_truncated, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- attention-side layers (no counterpart in the reference): what a head needs in which cells, queries or prompts attend to
+ * the maps of the networks above.  Inference only.  Element type float32 or bfloat16 (`dtype`: YOLO_DTYPE_*) for every
+ * activation and weight matrix; arithmetic, sums and softmax in float32, one rounding at the store.  Outputs must not overlap
+ * inputs; rows the outputs do not name are left as they were.  None allocates, synchronises or keeps anything between calls,
+ * so calls may overlap on any streams and may be captured into a HIP graph. */
+enum { YOLO_ACT_NONE = 0, YOLO_ACT_LEAKY = 1, YOLO_ACT_RELU = 2, YOLO_ACT_GELU = 3, YOLO_ACT_SILU = 4 };
+
+/* out[m,n] = act(sum_k x[m,k] * weight[n,k] + bias[n]) + residual[m,n]: the 1x1 conv2d of a feature map's cells (yolo_conv_forward)
+ * for weights that live in device memory, residual after the activation as there.  x [M,K], weight [N,K], residual / out [M,N], all
+ * row-major with row strides *_ld in elements; bias [N] (of `bias_dtype`) and residual may be NULL.  Leaky slope 0.1, gelu with
+ * the error function.  Rows on 16-byte boundaries with K a multiple of 8 (bf16) / 4 (f32) take the fast loads; any other
+ * stride, size or element-aligned pointer is accepted.  M = 0 is a no-op. */
+int yolo_linear(int dtype, const void* x, int64_t x_ld, const void* weight, int64_t weight_ld, const void* bias, int bias_dtype,
+                const void* residual, int64_t residual_ld, void* out, int64_t out_ld, int64_t M, int N, int K, int activation,
+                void* stream);
+
+/* Per (token, head) row h = x / sqrt(mean(x^2) + eps) * weight, then pair i of the first rotary_dim elements turned by
+ * position * frequencies[i]: pairs (i, i + rotary_dim/2), or (2i, 2i+1) if interleaved.  Queries and keys (of another length
+ * and head count) in one launch; k = NULL: queries only (a step over keys that are normalised already).
+ * q [B,Lq,Hq,D], k [B,Lk,Hk,D]: HOST *_strides = element strides of batch, token, head (last dimension contiguous);
+ * q_out, k_out packed.  *_weight [D] of `weight_dtype`, or NULL (ones).  frequencies: DEVICE float64 [rotary_dim/2], radians per position, or NULL
+ * (no rotation, positions unused).  *_positions: int32 (or int64: positions_int64) [L, axes], or [B, L, axes] if *_batched;
+ * with axes = 2 the first half of the pairs turns by coordinate 0, the second half by coordinate 1.  D <= 256, eps > 0. */
+int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const int64_t* q_strides, int Lq, int Hq, const void* q_weight,
+                      const void* q_positions, void* q_out, const void* k, const int64_t* k_strides, int Lk, int Hk,
+                      const void* k_weight, const void* k_positions, void* k_out, int weight_dtype, const double* frequencies,
+                      int rotary_dim, int axes, int positions_int64, int q_positions_batched, int k_positions_batched,
+                      int interleaved, float eps, void* stream);
+
+/* out = softmax(scale * q k^T) v: q [B,Lq,Hq,D] over k, v [B,Lk,Hk,D] of another length; query head h reads key head
+ * h / (Hq / Hk).  HOST *_strides as above, out [B,Lq,Hq,D] packed.  A key is kept when its index is below key_lens[b] (DEVICE int32
+ * [B], NULL: Lk; values are clamped to [0, Lk]) and key_mask[b,j] (DEVICE uint8 [B,Lk], NULL: all) is not 0; other keys have no
+ * influence whatever they hold.  A row without a kept key is zero (Lk = 0: all rows).  D <= 256, Hq a multiple of Hk.
+ * D a multiple of 8 with 16-byte aligned rows takes the matrix-core kernels; any other head size, stride or alignment is accepted. */
+size_t yolo_cross_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D);
+int yolo_cross_attention(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, const int32_t* key_lens, const uint8_t* key_mask, int B,
+                         int Lq, int Lk, int Hq, int Hk, int D, float scale, void* out, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,7 +12,7 @@ DTYPES = {"fp32": YOLO_DTYPE_F32, "float32": YOLO_DTYPE_F32, "f32": YOLO_DTYPE_F
           "bf16": YOLO_DTYPE_BF16, "bfloat16": YOLO_DTYPE_BF16}
 
 _c = ctypes
-_vp, _i, _f, _sz = _c.c_void_p, _c.c_int, _c.c_float, _c.c_size_t
+_vp, _i, _f, _sz, _i64 = _c.c_void_p, _c.c_int, _c.c_float, _c.c_size_t, _c.c_int64
 
 # name -> (restype, argtypes); every symbol declared in include/yolo_hip.h
 SIGNATURES = {
@@ -54,6 +54,10 @@ SIGNATURES = {
     "yolo_nms": (_i, [_vp, _vp, _i, _i, _i, _i, _f, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "yolo_pack_detections": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "yolo_nms_static": (_i, [_vp, _vp, _i, _i, _i, _i, _f, _f, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "yolo_linear": (_i, [_i, _vp, _i64, _vp, _i64, _vp, _i, _vp, _i64, _vp, _i64, _i64, _i, _i, _i, _vp]),
+    "yolo_qk_norm_rope": (_i, [_i, _i, _i] + [_vp, _vp, _i, _i, _vp, _vp, _vp] * 2 + [_i, _vp, _i, _i, _i, _i, _i, _i, _f, _vp]),
+    "yolo_cross_attention_workspace_bytes": (_sz, [_i] * 7),
+    "yolo_cross_attention": (_i, [_i] + [_vp] * 8 + [_i] * 6 + [_f, _vp, _vp, _sz, _vp]),
 }
 
 _lib = None

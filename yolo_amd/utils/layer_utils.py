@@ -7,6 +7,10 @@ TF creates a layer's variables when the layer function is called; here the varia
 `variable_scope(params)` - the eager counterpart of `tf.variable_scope` + `Saver.restore`.
 `yolov3.forward` does not go through these functions: it runs the whole fused plan
 (yolo_net_forward).  These exist for layer-level drop-in use and tests.
+
+`linear`, `qk_norm_rope` and `cross_attention` are the layers of a head in which cells, object queries or class prompts
+attend to the feature maps; the reference has none.  Their weights are tensors the caller keeps, and unlike the layers above
+they take and return bfloat16 as well as float32, without a cast at the boundary.
 """
 from __future__ import division, print_function
 
@@ -14,6 +18,7 @@ import contextlib
 import ctypes
 
 import numpy as np
+import torch
 
 from .. import _lib, _tensor
 
@@ -135,4 +140,226 @@ def upsample_layer(inputs, out_shape):
     else:
         _lib.check(_lib.lib().yolo_upsample_nearest(x.data_ptr(), B, H, W, C, new_height, new_width, out.data_ptr(),
                                                     _tensor.stream_ptr()))
+    return out
+
+
+# ---- layers over feature maps without a counterpart in the reference -------------------------------------------------------
+_DTYPE_CODES = {torch.float32: _lib.YOLO_DTYPE_F32, torch.bfloat16: _lib.YOLO_DTYPE_BF16}
+_ACTIVATIONS = {None: 0, "linear": 0, "leaky": 1, "relu": 2, "gelu": 3, "silu": 4}
+
+
+def _dev(x, name, dtype=None):
+    """numpy / torch (any device) -> tensor of its own type (or `dtype`) on the current GPU, strides kept."""
+    if not isinstance(x, torch.Tensor):
+        x = torch.from_numpy(np.asarray(x))
+        if x.dtype == torch.float64 and dtype is None:
+            x = x.float()
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient: yolo_amd implements the inference path only (call under torch.no_grad())" % name)
+    if dtype is not None and x.dtype != dtype:
+        x = x.to(dtype)
+    if not x.is_cuda or x.get_device() != torch.cuda.current_device():
+        x = x.to(_tensor.device())
+    return x
+
+
+def _code(x, name):
+    code = _DTYPE_CODES.get(x.dtype)
+    if code is None:
+        raise ValueError("%s must be float32 or bfloat16, got %s" % (name, x.dtype))
+    return code
+
+
+def _same_type(x, like, name):
+    if x.dtype != like.dtype:
+        raise ValueError("%s is %s, expected %s" % (name, x.dtype, like.dtype))
+    return x
+
+
+def _param(x, n, name):
+    """Bias / norm weight: [n] contiguous, float32 or bfloat16 -> (tensor or None, type code)."""
+    if x is None:
+        return None, 0
+    x = _dev(x, name)
+    if x.dim() != 1 or x.shape[0] != n:
+        raise ValueError("%s must be [%d], got %s" % (name, n, tuple(x.shape)))
+    return x.contiguous(), _code(x, name)
+
+
+def _rows(x):
+    """[..., n] -> (tensor, elements between rows) with all leading dimensions as rows of one stride; copied if there is none."""
+    n = x.shape[-1]
+    if x.is_contiguous():
+        return x, n
+    if x.dim() == 1:
+        return x.contiguous(), n
+    st, sh = x.stride(), x.shape
+    ok = n == 1 or st[-1] == 1
+    rows, ld = 1, None                                                # innermost row dimension of more than one row sets the stride
+    for i in range(x.dim() - 2, -1, -1):
+        if sh[i] == 1:
+            continue
+        if ld is None:
+            ld = st[i]
+        ok = ok and st[i] == rows * ld
+        rows *= sh[i]
+    if ok and (ld is None or ld >= n):
+        return x, n if ld is None else ld
+    return x.contiguous(), n
+
+
+def linear(inputs, weight, bias=None, activation=None, residual=None):
+    """act(inputs @ weight.T + bias) + residual in one launch: inputs [..., K] (a map's cells [B, H, W, K] as they are), weight
+    [N, K], bias [N], residual [..., N] -> [..., N], float32 or bfloat16 throughout (bias: either).  activation: None, "leaky"
+    (slope 0.1), "relu", "gelu" (error function) or "silu"; the residual is added after it, as in res_block.  yolo_linear."""
+    x, w = _dev(inputs, "inputs"), _dev(weight, "weight")
+    code = _code(x, "inputs")
+    _same_type(w, x, "weight")
+    if activation not in _ACTIVATIONS:
+        raise ValueError("linear: unknown activation %r" % (activation,))
+    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.shape[1] == 0 or w.shape[0] == 0:
+        raise ValueError("linear: inputs %s do not fit weight %s" % (tuple(x.shape), tuple(w.shape)))
+    N, K = int(w.shape[0]), int(w.shape[1])
+    b, bcode = _param(bias, N, "bias")
+    shape = x.shape[:-1] + (N,)
+    r, r_ld = None, 0
+    if residual is not None:
+        r = _same_type(_dev(residual, "residual"), x, "residual")
+        if r.shape != shape:
+            raise ValueError("linear: residual %s, expected %s" % (tuple(r.shape), tuple(shape)))
+        r, r_ld = _rows(r)
+    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    M = out.numel() // N
+    x, x_ld = _rows(x)
+    w, w_ld = _rows(w)
+    _lib.check(_lib.lib().yolo_linear(code, x.data_ptr(), x_ld, w.data_ptr(), w_ld, _tensor.ptr(b), bcode, _tensor.ptr(r), r_ld,
+                                      out.data_ptr(), N, M, N, K, _ACTIVATIONS[activation], _tensor.stream_ptr()))
+    return out
+
+
+def rope_frequencies(rotary_dim, base=10000.0, axes=1):
+    """float64 [rotary_dim / 2] on the current GPU, radians per position of every pair of `qk_norm_rope`: base ** (-i / n) for the
+    n = rotary_dim / 2 / axes pairs of an axis, the axes one after the other."""
+    if axes not in (1, 2) or rotary_dim <= 0 or rotary_dim % (2 * axes):
+        raise ValueError("rope_frequencies: rotary_dim %r does not split into pairs over %r axes" % (rotary_dim, axes))
+    n = rotary_dim // 2 // axes
+    f = float(base) ** (-np.arange(n, dtype=np.float64) / n)
+    return torch.from_numpy(np.tile(f, axes)).to(_tensor.device())
+
+
+def _heads(x, name):
+    """[B, L, H, D] with a contiguous last dimension -> (tensor, ctypes strides of batch, token, head)."""
+    if x.dim() != 4:
+        raise ValueError("%s must be [B, L, H, D], got %s" % (name, tuple(x.shape)))
+    st = x.stride()
+    if st[3] != 1 and x.shape[3] > 1:
+        x = x.contiguous()
+        st = x.stride()
+    return x, (ctypes.c_int64 * 3)(st[0], st[1], st[2])
+
+
+def _positions(p, B, L, axes, name):
+    """-> (contiguous tensor, batched).  [L] / [B, L] for one axis, [L, 2] / [B, L, 2] for two; a trailing 1 is allowed for one."""
+    p = _dev(p, name)
+    if p.dtype not in (torch.int32, torch.int64):
+        raise ValueError("%s must be int32 or int64, got %s" % (name, p.dtype))
+    shape = tuple(p.shape)
+    tail = () if axes == 1 and (shape == (L,) or shape == (B, L)) else (axes,)
+    if shape == (L,) + tail:
+        return p.contiguous(), 0
+    if shape == (B, L) + tail:
+        return p.contiguous(), 1
+    raise ValueError("%s %s fits neither %s nor %s" % (name, shape, (L,) + tail, (B, L) + tail))
+
+
+def qk_norm_rope(q, k, q_weight=None, k_weight=None, frequencies=None, q_positions=None, k_positions=None, eps=1e-6,
+                 interleaved=False, axes=None):
+    """Root-mean-square norm of every head of the queries and keys, then the rotation by position, in one launch:
+    q [B, Lq, Hq, D], k [B, Lk, Hk, D] (any strides over a contiguous D; None: queries only) -> new packed tensors (q, k).
+    *_weight [D] or None (ones).  frequencies: float64 [rotary_dim / 2] of `rope_frequencies` (None: no rotation); elements past
+    rotary_dim are normalised only.  Positions int32 / int64: [L] or [B, L]; for the cells of a map [L, 2] or [B, L, 2] (row,
+    column), where the first half of the pairs turns by the row and the second by the column.  `axes` (1 or 2) says which where
+    None would leave [B, L] = [L, 2] open.  Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) if `interleaved`.
+    yolo_qk_norm_rope."""
+    q, qs = _heads(_dev(q, "q"), "q")
+    code = _code(q, "q")
+    B, Lq, Hq, D = [int(v) for v in q.shape]
+    Lk, Hk, ks, ko = 0, 0, None, None
+    if k is not None:
+        k, ks = _heads(_same_type(_dev(k, "k"), q, "k"), "k")
+        Lk, Hk = int(k.shape[1]), int(k.shape[2])
+        if k.shape[0] != B or k.shape[3] != D:
+            raise ValueError("qk_norm_rope: k %s does not fit q %s" % (tuple(k.shape), tuple(q.shape)))
+        ko = torch.empty((B, Lk, Hk, D), dtype=q.dtype, device=q.device)
+    qw, qwc = _param(q_weight, D, "q_weight")
+    kw, kwc = _param(k_weight if k is not None else None, D, "k_weight")
+    if qw is not None and kw is not None and qwc != kwc:
+        raise ValueError("q_weight and k_weight must be of one type")
+    qp = kp = None
+    R, pos64, qb, kb = 0, 0, 0, 0
+    if frequencies is not None:
+        frequencies = _dev(frequencies, "frequencies", torch.float64).contiguous()
+        if frequencies.dim() != 1 or not 0 < 2 * frequencies.shape[0] <= D:
+            raise ValueError("qk_norm_rope: frequencies %s for heads of %d" % (tuple(frequencies.shape), D))
+        R = 2 * int(frequencies.shape[0])
+        if q_positions is None or (k is not None and k_positions is None):
+            raise ValueError("qk_norm_rope: frequencies need positions")
+        q_positions = _dev(q_positions, "q_positions")
+        if axes is None:
+            if tuple(q_positions.shape) == (2, 2) == (B, Lq):
+                raise ValueError("qk_norm_rope: positions [2, 2] of 2 x 2 queries may be one axis or two: pass axes")
+            axes = 2 if q_positions.dim() > 1 and q_positions.shape[-1] == 2 and tuple(q_positions.shape) != (B, Lq) else 1
+        if axes not in (1, 2) or R // 2 % axes:
+            raise ValueError("qk_norm_rope: %d pairs over %r axes" % (R // 2, axes))
+        qp, qb = _positions(q_positions, B, Lq, axes, "q_positions")
+        if k is not None:
+            kp, kb = _positions(k_positions, B, Lk, axes, "k_positions")
+            if kp.dtype != qp.dtype:
+                kp, qp = kp.long(), qp.long()
+        pos64 = int(qp.dtype == torch.int64)
+    qo = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    if D == 0 or Hq == 0 or (k is not None and Hk == 0):
+        raise ValueError("qk_norm_rope: no heads in q %s" % (tuple(q.shape),))
+    _lib.check(_lib.lib().yolo_qk_norm_rope(
+        code, B, D, q.data_ptr(), qs, Lq, Hq, _tensor.ptr(qw), _tensor.ptr(qp), qo.data_ptr(),
+        _tensor.ptr(k), ks, Lk, Hk, _tensor.ptr(kw), _tensor.ptr(kp), _tensor.ptr(ko), qwc if qw is not None else kwc,
+        _tensor.ptr(frequencies), R, axes or 1, pos64, qb, kb, int(bool(interleaved)), float(eps), _tensor.stream_ptr()))
+    return qo, ko
+
+
+def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
+    """softmax(scale * q k^T) v: q [B, Lq, Hq, D] over the states k, v [B, Lk, Hk, D] of another length (any strides over a
+    contiguous D, so the halves of one key / value projection go in as views); Hq a multiple of Hk, query head h reads key head
+    h // (Hq // Hk).  key_lens [B] int32: keys from key_lens[b] on are padding; key_mask [B, Lk] bool: False leaves a key out.
+    What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.
+    -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
+    q, qs = _heads(_dev(q, "q"), "q")
+    code = _code(q, "q")
+    k, ks = _heads(_same_type(_dev(k, "k"), q, "k"), "k")
+    v, vs = _heads(_same_type(_dev(v, "v"), q, "v"), "v")
+    B, Lq, Hq, D = [int(n) for n in q.shape]
+    Lk, Hk = int(k.shape[1]), int(k.shape[2])
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
+    if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
+        raise ValueError("cross_attention: %d query heads over %d key heads of %d" % (Hq, Hk, D))
+    if key_lens is not None:
+        key_lens = _dev(key_lens, "key_lens")
+        if tuple(key_lens.shape) != (B,) or key_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError("key_lens must be int32 [%d], got %s %s" % (B, key_lens.dtype, tuple(key_lens.shape)))
+        if key_lens.dtype == torch.int64:
+            key_lens = key_lens.clamp(0, Lk).to(torch.int32)
+        key_lens = key_lens.contiguous()
+    if key_mask is not None:
+        key_mask = _dev(key_mask, "key_mask")
+        if tuple(key_mask.shape) != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8):
+            raise ValueError("key_mask must be bool [%d, %d], got %s %s" % (B, Lk, key_mask.dtype, tuple(key_mask.shape)))
+        key_mask = key_mask.contiguous()
+    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    L = _lib.lib()
+    need = L.yolo_cross_attention_workspace_bytes(code, B, Lq, Lk, Hq, Hk, D)
+    ws = _tensor.workspace(need) if need else None
+    _lib.check(L.yolo_cross_attention(code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _tensor.ptr(key_lens),
+                                      _tensor.ptr(key_mask), B, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None else float(scale),
+                                      out.data_ptr(), _tensor.ptr(ws), need, _tensor.stream_ptr()))
     return out
