@@ -5,6 +5,9 @@
 // o <- o exp(m - m') + sum exp(s - m') v and l likewise, result o / l.  Scores, m, l and o are f32.  A key is kept when its
 // index is below key_lens[b] and its key_mask byte is set; what is not kept is never multiplied (its score is replaced, its
 // value row not used), so that infinities and NaN there stay out.  A row without a kept key is zero.
+#include <cmath>
+#include <type_traits>
+
 #include "layer_common.h"
 
 namespace yolo {
@@ -19,6 +22,12 @@ struct AttnK {
     long long qb, ql, qh, kb, kl, kh, vb, vl, vh;   // element strides
     int B, Lq, Lk, Hq, Hk, D, G;        // G = Hq / Hk
     float scale;
+    // matrix-core kernels
+    uint32_t q_and, q_xor;              // applied to every 32 bits of q: a negative or zero scale is folded into q
+    float scale2;                       // |scale| * log2(e) (log2(e) for scale 0): weights are 2^(scale2 * (s - max))
+    int rtiles, splits, tps;            // row tiles per (image, key head), key splits, key tiles per split
+    float* part;                        // [splits][B*Lq*Hq][D] unnormalised results
+    float2* ml;                         // [splits][B*Lq*Hq] (maximum, sum); sum -1: no kept key in the split
 };
 
 // keys of image b that can be kept: [0, n)
@@ -98,11 +107,433 @@ __global__ __launch_bounds__(256) void cross_attention_general_kernel(AttnK p) {
     }
 }
 
+// ---- tiles on the matrix cores --------------------------------------------------------------------------------------------------
+// A workgroup of WAVES waves takes 32 NQ WAVES query rows of one (image, key head) - row r is query r / G, head r % G of the group,
+// so that the heads that share k and v share their tiles - and walks KT keys at a time; k and v tiles are double-buffered in
+// LDS by DMA, one barrier per tile.
+//
+// Scores are computed transposed, S^T = K Q^T on 32x32 MFMAs: lane l then holds 16 scores of ONE query (l % 32) per 32 keys (keys
+// 8 b + 4 (l / 32) + i at register 4 b + i), so maximum and sum are in-lane but for one exchange with lane l ^ 32, and the
+// rescaling factor of o is a lane's own scalar.  P^T in that layout IS the second operand of O^T = V^T P^T if the reduction
+// index runs over the keys in the order the lane holds them; v is read to match: bf16 by ds_read_b64_tr_b16 (4 keys x 16
+// elements transposed per 16 lanes), f32 by single words.
+//
+// The running maximum is only raised when a score exceeds it by 2^8 in weight: weights stay below 2^8, which costs no precision
+// (they are floating point) and most tiles skip the rescaling of o.
+// bf16: the weights are rounded to bf16 for the second product, at most 2^-9 of each, independent in sign, which is of the size of the
+// rounding of the result; their sum is taken of the f32 values.
+//
+// LDS rows are the next power of two of the head size.  k: 16-byte piece c of a row at c ^ f(row) so that 16 rows' pieces fall on
+// all banks; v: 64-byte (f32: 128-byte) blocks exchanged likewise for the transposed reads of four rows at a time.
+__device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
+
+template <bool BF16, int DC> struct AttnTile {
+    static constexpr int Z = BF16 ? 2 : 4, P = 16 / Z;                              // bytes and elements of a piece
+    static constexpr int ROW = DC * Z <= 64 ? 64 : DC * Z <= 128 ? 128 : DC * Z <= 256 ? 256 : DC * Z <= 512 ? 512 : 1024;
+    static constexpr int PCS = ROW / 16, KT = ROW > 512 ? 32 : 64;                  // pieces of an LDS row, keys per tile
+    static constexpr int RPL = ROW >= 256 ? 1 : 256 / ROW;                          // rows per 256 bytes (all banks)
+    static constexpr int TILE = KT * ROW;                                           // bytes of one k or v tile
+    static constexpr int LDS = 4 * TILE;
+    static constexpr int BLK = BF16 ? 4 : 8;                                        // pieces of a v block
+    static __device__ __forceinline__ int kpiece(int row, int c) { return c ^ ((row / RPL) & (PCS - 1)); }
+    static __device__ __forceinline__ int vpiece(int row, int c) {
+        constexpr int NB = PCS / BLK;                                               // blocks of a row
+        if constexpr (NB <= 1) return c;
+        else if constexpr (BF16) return c ^ ((((row & 3) / RPL) & (NB - 1)) * BLK);
+        else return c ^ (((row >> 2) & 1) * BLK);
+    }
+};
+
+template <bool BF16, int DC, int WAVES, int NQ>
+__global__ __launch_bounds__(WAVES * 64) void cross_attention_tile_kernel(AttnK p) {
+    typedef typename Elem<BF16>::type T;
+    typedef AttnTile<BF16, DC> L;
+    constexpr int P = L::P, PCS = L::PCS, KT = L::KT, NT = WAVES * 64;
+    constexpr int QS = DC / (2 * P);                        // k steps of S: two pieces (one per lane half) each
+    constexpr int DT = DC / 32, KB = KT / 32;               // 32-wide tiles of o, 32-key tiles of S
+    constexpr int RPI = NT / PCS;                           // rows a pass of all threads stages
+    constexpr int NI = KT / RPI;
+    static_assert(KT % RPI == 0, "whole passes");
+    extern __shared__ char lds[];                           // k0 k1 v0 v1
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, half = lane >> 5;
+    unsigned id = xcd_chunk(blockIdx.x, gridDim.x);
+    const int rt = (int)(id % p.rtiles);
+    id /= p.rtiles;
+    const int split = (int)(id % p.splits);
+    id /= p.splits;
+    const int hk = (int)(id % p.Hk), b = (int)(id / p.Hk);
+    const int rows = p.Lq * p.G;
+    const int n = key_count(p, b);
+    const int t0 = split * p.tps;
+    const int t1 = min((n + KT - 1) / KT, t0 + p.tps);
+
+    // query rows of this wave -> registers (operand layout: column = row of q, 16-byte piece 2 step + half)
+    int row[NQ];
+    long long orow[NQ];                                     // row of the packed output
+    u32x4 fq[NQ][QS];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+        row[x] = rt * (32 * NQ * WAVES) + (wave * NQ + x) * 32 + col;
+        const int r = min(row[x], rows - 1);
+        const int l = r / p.G, h = hk * p.G + r % p.G;
+        orow[x] = ((long long)b * p.Lq + l) * p.Hq + h;
+        const char* q = p.q + (b * p.qb + l * p.ql + h * p.qh) * (long long)sizeof(T);
+#pragma unroll
+        for (int s = 0; s < QS; ++s) {
+            const int c = 2 * s + half;
+            u32x4 v = *(c * P < p.D ? (const u32x4*)(q + c * 16) : &kZeroPiece);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = (v[j] & p.q_and) ^ p.q_xor;
+            fq[x][s] = v;
+        }
+    }
+
+    f32x16 o[NQ][DT];
+    float mref[NQ], sum[NQ];
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+        mref[x] = -__builtin_inff();
+        sum[x] = 0.f;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[x][i][r] = 0.f;
+    }
+
+    // staging: thread covers slot tid % PCS of rows tid / PCS + RPI i
+    const int r0 = tid / PCS, slot = tid % PCS;
+    const long long kls = p.kl * (long long)sizeof(T), vls = p.vl * (long long)sizeof(T);
+    const char* kbase = p.k + (b * p.kb + hk * p.kh) * (long long)sizeof(T);
+    const char* vbase = p.v + (b * p.vb + hk * p.vh) * (long long)sizeof(T);
+    const uint8_t* mrow = p.mask ? p.mask + (long long)b * p.Lk : nullptr;
+    auto mask_byte = [&](int t) {                           // lane = key of tile t; 0 beyond the last key
+        const int j = t * KT + lane;
+        return (mrow && lane < KT && j < n) ? (int)mrow[j] : 0;
+    };
+    auto kept_bits = [&](int t, int mb) -> unsigned long long {
+        if (mrow) return __ballot(mb != 0);
+        const int left = n - t * KT;
+        return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1ull;
+    };
+    const unsigned long long full = KT == 64 ? ~0ull : 0xffffffffull;
+    const bool padded = p.D * L::Z != L::ROW;
+    auto issue = [&](int t, int buf, unsigned long long kept) {
+        char* kd = lds + buf * L::TILE + wave * 1024;
+        char* vd = lds + (2 + buf) * L::TILE + wave * 1024;
+        const char* ks = kbase + ((long long)t * KT + r0) * kls;
+        const char* vs = vbase + ((long long)t * KT + r0) * vls;
+        const bool plain = !padded && (kept & full) == full;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const int r = r0 + i * RPI;
+            const int kc = L::kpiece(r, slot), vc = L::vpiece(r, slot);
+            const char* kg = ks + (long long)(i * RPI) * kls + kc * 16;
+            const char* vg = vs + (long long)(i * RPI) * vls + vc * 16;
+            if (!plain) {
+                const bool in = (kept >> r) & 1;
+                if (!in || kc * P >= p.D) kg = (const char*)&kZeroPiece;
+                if (!in || vc * P >= p.D) vg = (const char*)&kZeroPiece;
+            }
+            dma16(kg, kd + i * NT * 16);
+            dma16(vg, vd + i * NT * 16);
+        }
+    };
+
+    bool any = false;
+    unsigned long long kept = 0;
+    int mb = 0;
+    if (t0 < t1) {
+        kept = kept_bits(t0, mask_byte(t0));
+        issue(t0, 0, kept);
+        mb = mask_byte(t0 + 1);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
+        const unsigned long long next = kept_bits(t + 1, mb);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (t + 1 < t1) {
+            issue(t + 1, buf ^ 1, next);
+            mb = mask_byte(t + 2);
+        }
+        const char* kt = lds + buf * L::TILE;
+        const char* vt = lds + (2 + buf) * L::TILE;
+
+        f32x16 s[NQ][KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int x = 0; x < NQ; ++x)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[x][kb][r] = 0.f;
+            const int key = kb * 32 + col;
+#pragma unroll
+            for (int st = 0; st < QS; ++st) {
+                const u32x4 fk = *(const u32x4*)(kt + key * L::ROW + L::kpiece(key, 2 * st + half) * 16);
+#pragma unroll
+                for (int x = 0; x < NQ; ++x) {
+                    if constexpr (BF16) {
+                        s[x][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fk), __builtin_bit_cast(bf16x8, fq[x][st]), s[x][kb], 0, 0, 0);
+                    } else {
+                        const f32x4 a = __builtin_bit_cast(f32x4, fk), q = __builtin_bit_cast(f32x4, fq[x][st]);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) s[x][kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], q[j], s[x][kb], 0, 0, 0);
+                    }
+                }
+            }
+        }
+        if ((kept & full) != full) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool in = (kept >> (kb * 32 + 8 * (r >> 2) + 4 * half + (r & 3))) & 1;
+#pragma unroll
+                    for (int x = 0; x < NQ; ++x) s[x][kb][r] = in ? s[x][kb][r] : -__builtin_inff();
+                }
+        }
+        any |= kept != 0;
+        kept = next;
+
+#pragma unroll
+        for (int x = 0; x < NQ; ++x) {
+            float mt = s[x][0][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[x][kb][r]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const bool raise = (mt - mref[x]) * p.scale2 > 8.f;                     // false while both are -inf
+            if (__any(raise)) {
+                const float mn = fmaxf(mref[x], mt);
+                const float c = mref[x] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mref[x] - mn) * p.scale2);
+                mref[x] = mn;
+                sum[x] *= c;
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[x][i][r] *= c;
+            }
+            const float base = mref[x] == -__builtin_inff() ? 0.f : mref[x] * p.scale2;
+            float st = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][kb][r], p.scale2, -base));
+                    s[x][kb][r] = e;
+                    st += e;
+                }
+            sum[x] += st;
+        }
+
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            if constexpr (BF16) {
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {               // 16 keys: registers 8 g .. 8 g + 7
+                    bf16x8 fp[NQ];
+#pragma unroll
+                    for (int x = 0; x < NQ; ++x) {
+                        u32x4 pk;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(s[x][kb][8 * g + 2 * j], s[x][kb][8 * g + 2 * j + 1]);
+                        fp[x] = __builtin_bit_cast(bf16x8, pk);
+                    }
+                    // lane's address for the transposed read: key row (lane / 4) % 4 of its four keys, 4 elements at 4 (lane % 4)
+                    const int key = kb * 32 + 16 * g + 4 * half + ((lane >> 2) & 3);
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        const int e = i * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;             // first element
+                        const int c = e / 8, w = (e & 7) * 2;
+                        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+                            (__attribute__((address_space(3))) char*)vt + key * L::ROW + L::vpiece(key, c) * 16 + w));
+                        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+                            (__attribute__((address_space(3))) char*)vt + (key + 8) * L::ROW + L::vpiece(key + 8, c) * 16 + w));
+                        typedef short s16x8 __attribute__((ext_vector_type(8)));
+                        const bf16x8 fv = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int x = 0; x < NQ; ++x) o[x][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv, fp[x], o[x][i], 0, 0, 0);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = kb * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+                    for (int i = 0; i < DT; ++i) {
+                        const int e = i * 32 + col;
+                        const float fv = *(const float*)(vt + key * L::ROW + L::vpiece(key, e / 4) * 16 + (e & 3) * 4);
+#pragma unroll
+                        for (int x = 0; x < NQ; ++x) o[x][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(fv, s[x][kb][r], o[x][i], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+
+    const long long total = (long long)p.B * p.Lq * p.Hq;
+#pragma unroll
+    for (int x = 0; x < NQ; ++x) {
+        const float l = sum[x] + __shfl_xor(sum[x], 32);
+        const bool in = row[x] < rows;
+        const bool parts = p.part != nullptr;
+        const float f = parts ? 1.0f : any ? 1.0f / l : 0.f;
+        if (in && parts && half == 0) p.ml[split * total + orow[x]] = make_float2(mref[x], any ? l : -1.0f);
+#pragma unroll
+        for (int i = 0; i < DT; ++i) {
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                // registers 8 g + 0..3 and 8 g + 4..7 are elements 16 g + 4 half + 0..3 and + 8: after the exchange of lane halves a lane
+                // holds 8 consecutive elements, 16 g + 8 half ..
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float a = o[x][i][8 * g + j] * f, c = o[x][i][8 * g + 4 + j] * f;
+                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(c), false, false);
+                    v[j] = __uint_as_float(sw[0]);
+                    v[4 + j] = __uint_as_float(sw[1]);
+                }
+                const int d = i * 32 + 16 * g + 8 * half;
+                if (!in || d >= p.D) continue;              // D is whole groups of 8
+                if (parts || !BF16) {
+                    float* dst = parts ? p.part + (split * total + orow[x]) * p.D + d : (float*)p.out + orow[x] * p.D + d;
+                    *(f32x4*)dst = f32x4{v[0], v[1], v[2], v[3]};
+                    *(f32x4*)(dst + 4) = f32x4{v[4], v[5], v[6], v[7]};
+                } else {
+                    u32x4 pk;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                    *(u32x4*)((__bf16*)p.out + orow[x] * p.D + d) = pk;
+                }
+            }
+        }
+    }
+}
+
+// Joins the key splits of a row: one wave per row, lane = split for the maxima and sums, lane + 64 i = element for the results.
+// The splits are added in order: the result does not depend on the launch.
+constexpr int kMaxSplits = 64;
+
+template <bool BF16>
+__global__ __launch_bounds__(256) void cross_attention_join_kernel(AttnK p) {
+    typedef typename Elem<BF16>::type T;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long long total = (long long)p.B * p.Lq * p.Hq;
+    const long long row = (long long)blockIdx.x * 4 + wave;
+    if (row >= total) return;
+    const bool have = lane < p.splits;
+    const float2 ml = have ? p.ml[lane * total + row] : make_float2(-__builtin_inff(), -1.0f);
+    const bool kept = have && ml.y != -1.0f;                // a NaN sum is kept
+    const bool any = __ballot(kept) != 0;
+    float m = kept ? ml.x : -__builtin_inff();
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    // a split whose kept scores are all -inf has maximum -inf, sum 0 and results 0
+    float w = kept && ml.x != -__builtin_inff() ? __builtin_amdgcn_exp2f((ml.x - m) * p.scale2) : kept && ml.y == 0.f ? 0.f : kept ? 1.f : 0.f;
+    float l = kept ? w * ml.y : 0.f;
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < p.splits; ++s) {
+        const float ws = __shfl(w, s);
+        if (!__shfl((int)kept, s)) continue;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int d = lane + 64 * i;
+            if (d < p.D) o[i] = __builtin_fmaf(ws, p.part[(s * total + row) * p.D + d], o[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 64 * i;
+        if (d < p.D) ((T*)p.out)[row * p.D + d] = (T)(any ? o[i] / l : 0.f);
+    }
+}
+
+// ---- plan: the tile shape and the number of key splits, by sizes and type alone ---------------------------------------------------
+struct AttnPlan {
+    int dc, waves, nq, kt, rtiles, splits, tps;
+    size_t bytes;
+};
+
+static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
+    AttnPlan a;
+    const int z = dtype == YOLO_DTYPE_BF16 ? 2 : 4;
+    a.dc = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
+    a.kt = a.dc * z > 512 ? 32 : 64;
+    const long long rows = (long long)Lq * (Hq / Hk);
+    a.waves = rows <= 32 ? 1 : 4;
+    a.nq = 1;
+    a.rtiles = (int)((rows + 32 * a.waves * a.nq - 1) / (32 * a.waves * a.nq));
+    const long long blocks = (long long)a.rtiles * B * Hk;
+    const int tiles = (Lk + a.kt - 1) / a.kt;
+    // few row tiles: the keys are split until there are about 512 workgroups (1024 of one wave)
+    const long long want = a.waves == 1 ? 1024 : 512;
+    long long s = blocks >= want / 2 ? 1 : want / blocks;
+    if (s > tiles) s = tiles;
+    if (s > kMaxSplits) s = kMaxSplits;
+    if (s < 1) s = 1;
+    a.tps = tiles ? (int)((tiles + s - 1) / s) : 0;
+    a.splits = a.tps ? (tiles + a.tps - 1) / a.tps : 1;
+    a.bytes = a.splits > 1 ? (size_t)a.splits * B * Lq * Hq * (D + 2) * 4 : 0;
+    return a;
+}
+
+template <bool BF16, int DC, int WAVES, int NQ>
+static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
+    constexpr int kLds = AttnTile<BF16, DC>::LDS;
+    if (kLds > 64 * 1024) {
+        static std::atomic<bool> attr_done[16];   // setting the attribute twice is harmless, the flag only must not tear
+        int dev = 0;
+        YOLO_HIP_CHECK(hipGetDevice(&dev));
+        if (dev >= 16 || !attr_done[dev]) {
+            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, NQ>,
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+            if (dev < 16) attr_done[dev] = true;
+        }
+    }
+    const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk;
+    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 workgroups");
+    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, NQ>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
+    YOLO_HIP_CHECK(hipGetLastError());
+    return YOLO_OK;
+}
+
+template <bool BF16, int DC>
+static int launch_attn_dc(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
+    if (a.waves == 1) return launch_attn_tile<BF16, DC, 1, 1>(p, stream);
+    return launch_attn_tile<BF16, DC, 4, 1>(p, stream);
+}
+
+template <bool BF16>
+static int launch_attn(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
+    int rc;
+    switch (a.dc) {
+        case 32: rc = launch_attn_dc<BF16, 32>(p, a, stream); break;
+        case 64: rc = launch_attn_dc<BF16, 64>(p, a, stream); break;
+        case 96: rc = launch_attn_dc<BF16, 96>(p, a, stream); break;
+        case 128: rc = launch_attn_dc<BF16, 128>(p, a, stream); break;
+        default: rc = launch_attn_dc<BF16, 256>(p, a, stream); break;
+    }
+    if (rc != YOLO_OK || p.splits == 1) return rc;
+    const unsigned long long blocks = ((unsigned long long)p.B * p.Lq * p.Hq + 3) / 4;
+    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^33 rows");
+    hipLaunchKernelGGL(cross_attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    YOLO_HIP_CHECK(hipGetLastError());
+    return YOLO_OK;
+}
+
 }  // namespace yolo
 
 extern "C" size_t yolo_cross_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
-    (void)dtype; (void)B; (void)Lq; (void)Lk; (void)Hq; (void)Hk; (void)D;
-    return 0;
+    using namespace yolo;
+    if ((dtype != YOLO_DTYPE_F32 && dtype != YOLO_DTYPE_BF16) || B <= 0 || Lq <= 0 || Lk <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
+        D <= 0 || D > 256 || D % 8 || (unsigned long long)B * Lq >= (1ull << 31) || Hq > 65536 || (long long)Lq * (Hq / Hk) >= (1ll << 31))
+        return 0;
+    return attn_plan(dtype, B, Lq, Lk, Hq, Hk, D).bytes;
 }
 
 extern "C" int yolo_cross_attention(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -120,7 +551,7 @@ extern "C" int yolo_cross_attention(int dtype, const void* q, const int64_t* q_s
     YOLO_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (z - 1)) == 0 && ((uintptr_t)key_lens & 3) == 0,
                  YOLO_ERR_ARG, "cross_attention: a pointer is not aligned to its element");
     YOLO_REQUIRE((unsigned long long)B * Lq < (1ull << 31) && Hq <= 65536, YOLO_ERR_UNSUPPORTED, "cross_attention: B * Lq must be below 2^31, at most 65536 heads");
-    (void)workspace; (void)workspace_bytes;
+    YOLO_REQUIRE(std::isfinite(scale), YOLO_ERR_ARG, "cross_attention: scale must be finite");
     AttnK p;
     p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.out = (char*)out;
     p.lens = key_lens; p.mask = key_mask;
@@ -131,6 +562,27 @@ extern "C" int yolo_cross_attention(int dtype, const void* q, const int64_t* q_s
         p.vb = v_strides[0]; p.vl = v_strides[1]; p.vh = v_strides[2];
     }
     p.B = B; p.Lq = Lq; p.Lk = Lk; p.Hq = Hq; p.Hk = Hk; p.D = D; p.G = Hq / Hk; p.scale = scale;
+    p.part = nullptr; p.ml = nullptr; p.q_and = ~0u; p.q_xor = 0; p.scale2 = 0.f; p.rtiles = 0; p.splits = 1; p.tps = 0;
+    // the matrix-core kernels read whole 16-byte pieces of rows and hold the rows of a head group in 32 bits
+    bool fast = Lk > 0 && D % 8 == 0 && aligned16(out) && (long long)Lq * p.G < (1ll << 31);
+    const void* base[3] = {q, k, v};
+    const int64_t* st[3] = {q_strides, k_strides, v_strides};
+    for (int i = 0; fast && i < 3; ++i)
+        fast = aligned16(base[i]) && st[i][0] * z % 16 == 0 && st[i][1] * z % 16 == 0 && st[i][2] * z % 16 == 0;
+    if (fast) {
+        const AttnPlan a = attn_plan(dtype, B, Lq, Lk, Hq, Hk, D);
+        p.rtiles = a.rtiles; p.splits = a.splits; p.tps = a.tps;
+        p.scale2 = scale == 0.f ? 1.44269504f : std::fabs(scale) * 1.44269504f;
+        p.q_and = scale == 0.f ? 0u : ~0u;
+        p.q_xor = scale < 0.f ? (dtype == YOLO_DTYPE_BF16 ? 0x80008000u : 0x80000000u) : 0u;
+        if (a.splits > 1) {
+            YOLO_REQUIRE(workspace && workspace_bytes >= a.bytes && aligned16(workspace), YOLO_ERR_WORKSPACE,
+                         "cross_attention: workspace of %zu bytes (16-byte aligned) needed, got %zu", a.bytes, workspace ? workspace_bytes : (size_t)0);
+            p.part = (float*)workspace;
+            p.ml = (float2*)(p.part + (size_t)a.splits * B * Lq * Hq * D);
+        }
+        return dtype == YOLO_DTYPE_BF16 ? launch_attn<true>(p, a, (hipStream_t)stream) : launch_attn<false>(p, a, (hipStream_t)stream);
+    }
     const unsigned long long blocks = ((unsigned long long)B * Lq * Hq + 3) / 4;
     YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^33 rows");
     if (dtype == YOLO_DTYPE_BF16) hipLaunchKernelGGL(cross_attention_general_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p);
