@@ -106,6 +106,129 @@ __global__ __launch_bounds__(256) void qk_norm_rope_general_kernel(RopeK p) {
     }
 }
 
+// The usual layout: rotary_dim = D (or no rotation), D whole pairs of 16-byte pieces, aligned rows.  A lane holds two pieces whose
+// elements are each other's partners - pieces c and c + D/2 of a row, or neighbours if interleaved - so that the rotation needs no
+// exchange; LPR = D / (2 pieces) lanes, rounded up to a power of two, make a row, and its sum of squares is log2(LPR) lane exchanges.
+// Bandwidth bounds it: a workgroup issues its first row loads before it computes the table (one sine / cosine per thread or so,
+// shared by all heads of a token).
+template <bool BF16>
+__device__ __forceinline__ void unpack_piece(u32x4 v, float* f) {
+    if constexpr (BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f[2 * j] = bf16_lo(v[j]);
+            f[2 * j + 1] = bf16_hi(v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(v[j]);
+    }
+}
+
+template <bool BF16>
+__device__ __forceinline__ u32x4 pack_piece(const float* f) {
+    u32x4 v;
+    if constexpr (BF16) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = pack_bf16(f[2 * j], f[2 * j + 1]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = __float_as_uint(f[j]);
+    }
+    return v;
+}
+
+template <bool BF16, int LPR, bool IL>
+__global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeK p) {
+    typedef typename Elem<BF16>::type T;
+    constexpr int P = Elem<BF16>::kPiece, RPP = 256 / LPR;     // rows a pass of the workgroup covers
+    __shared__ float2 cs[kRopeTable];
+    __shared__ float wt[256];
+    const bool second = blockIdx.x >= p.blocks0;
+    const RopeSide& s = p.side[second];
+    const int t0 = (int)(blockIdx.x - (second ? p.blocks0 : 0)) * s.tpb;
+    const int nt = min(s.tpb, s.tokens - t0), rows = nt * s.H;
+    const int c = threadIdx.x % LPR, rw = threadIdx.x / LPR;
+    const bool lane_in = c * 2 * P < p.D;                       // D / (2 P) lanes of the LPR hold pieces
+    const int da = IL ? 2 * c * P : c * P, db = IL ? da + P : da + p.D / 2;
+    u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    int tl = 0, h = 0;
+    auto load = [&](int r) {
+        a = b = u32x4{0, 0, 0, 0};
+        if (r >= rows || !lane_in) return;
+        tl = r / s.H;
+        h = r - tl * s.H;
+        const int t = t0 + tl, bi = t / s.L;
+        const T* x = (const T*)s.x + bi * s.sb + (t - bi * s.L) * s.sl + h * s.sh;
+        a = *(const u32x4*)(x + da);
+        b = *(const u32x4*)(x + db);
+    };
+    load(rw);
+    rope_tables(p, s, t0, nt, cs, wt);
+    __syncthreads();
+    float wa[P], wb[P];
+    if (lane_in) {
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            wa[j] = wt[da + j];
+            wb[j] = wt[db + j];
+        }
+    }
+    for (int r = rw; r < rows + rw; r += RPP) {                 // every lane of a wave makes the same trips: r - rw is uniform
+        float u[P], v[P], ss = 0.f;
+        unpack_piece<BF16>(a, u);
+        unpack_piece<BF16>(b, v);
+        const int tc = tl, hc = h;
+        const bool in = r < rows && lane_in;
+        if (r + RPP < rows) load(r + RPP);                      // the next row is on its way while this one is computed
+#pragma unroll
+        for (int j = 0; j < P; ++j) ss = __builtin_fmaf(u[j], u[j], __builtin_fmaf(v[j], v[j], ss));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+        if (!in) continue;
+        const float rs = 1.0f / sqrtf(ss / (float)p.D + p.eps);
+#pragma unroll
+        for (int j = 0; j < P; ++j) {
+            u[j] *= rs * wa[j];
+            v[j] *= rs * wb[j];
+        }
+        if (p.freq) {
+            const float2* t = cs + tc * (p.D / 2) + c * P;      // pairs c P .. c P + P - 1 in either layout
+#pragma unroll
+            for (int j = 0; j < P; ++j) {
+                const float2 w = t[j];
+                float& x = IL ? (2 * j < P ? u[(2 * j) % P] : v[(2 * j) % P]) : u[j];
+                float& y = IL ? (2 * j < P ? u[(2 * j) % P + 1] : v[(2 * j) % P + 1]) : v[j];
+                const float x0 = x, y0 = y;
+                x = __builtin_fmaf(-y0, w.y, x0 * w.x);
+                y = __builtin_fmaf(x0, w.y, y0 * w.x);
+            }
+        }
+        T* o = (T*)s.out + ((long long)(t0 + tc) * s.H + hc) * p.D;
+        *(u32x4*)(o + da) = pack_piece<BF16>(u);
+        *(u32x4*)(o + db) = pack_piece<BF16>(v);
+    }
+}
+
+template <bool BF16, int LPR>
+static void launch_rope_rows(const RopeK& p, unsigned blocks, hipStream_t stream) {
+    if (p.interleaved) hipLaunchKernelGGL((qk_norm_rope_kernel<BF16, LPR, true>), dim3(blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((qk_norm_rope_kernel<BF16, LPR, false>), dim3(blocks), dim3(256), 0, stream, p);
+}
+
+template <bool BF16>
+static void launch_rope(const RopeK& p, int lpr, unsigned blocks, hipStream_t stream) {
+    switch (lpr) {
+        case 1: launch_rope_rows<BF16, 1>(p, blocks, stream); break;
+        case 2: launch_rope_rows<BF16, 2>(p, blocks, stream); break;
+        case 4: launch_rope_rows<BF16, 4>(p, blocks, stream); break;
+        case 8: launch_rope_rows<BF16, 8>(p, blocks, stream); break;
+        case 16: launch_rope_rows<BF16, 16>(p, blocks, stream); break;
+        case 32: launch_rope_rows<BF16, 32>(p, blocks, stream); break;
+        default: hipLaunchKernelGGL(qk_norm_rope_general_kernel<BF16>, dim3(blocks), dim3(256), 0, stream, p);
+    }
+}
+
 }  // namespace yolo
 
 extern "C" int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const int64_t* q_strides, int Lq, int Hq,
@@ -131,6 +254,17 @@ extern "C" int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const i
     p.D = D; p.R = rotary_dim; p.axes = axes; p.interleaved = interleaved != 0; p.w_bf16 = weight_dtype == YOLO_DTYPE_BF16;
     p.pos64 = positions_int64 != 0; p.freq = frequencies; p.eps = eps;
     const int z = dtype == YOLO_DTYPE_BF16 ? 2 : 4;
+    const int piece = 16 / z;
+    // lanes per row of the register kernel, 0: general kernel
+    int lpr = 0;
+    if (D % (2 * piece) == 0 && (rotary_dim == 0 || rotary_dim == D))
+        for (lpr = 1; lpr * 2 * piece < D;) lpr *= 2;
+    for (int i = 0; i < 2 && lpr; ++i) {
+        const int64_t* st = i ? k_strides : q_strides;
+        const void* x = i ? k : q;
+        if (!x || !st) continue;
+        if (!aligned16(x) || !aligned16(i ? k_out : q_out) || st[0] * z % 16 || st[1] * z % 16 || st[2] * z % 16) lpr = 0;
+    }
     unsigned long long blocks[2] = {0, 0};
     for (int i = 0; i < 2; ++i) {
         RopeSide& s = p.side[i];
@@ -148,7 +282,7 @@ extern "C" int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const i
         YOLO_REQUIRE((long long)B * s.L < (1ll << 31) && s.H <= 65536, YOLO_ERR_UNSUPPORTED, "qk_norm_rope: B * L must be below 2^31, at most 65536 heads");
         s.sb = st[0]; s.sl = st[1]; s.sh = st[2];
         s.tokens = B * s.L;
-        s.tpb = 32 / s.H;
+        s.tpb = (lpr ? 2 * 256 / lpr : 32) / s.H;              // two rows for every lane group
         if (s.tpb < 1) s.tpb = 1;
         if (p.R && s.tpb > kRopeTable / (p.R / 2)) s.tpb = kRopeTable / (p.R / 2);
         blocks[i] = ((unsigned long long)s.tokens + s.tpb - 1) / s.tpb;
@@ -157,8 +291,8 @@ extern "C" int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const i
     if (total == 0) return YOLO_OK;
     YOLO_REQUIRE(total < (1ull << 31), YOLO_ERR_UNSUPPORTED, "qk_norm_rope: more than 2^31 workgroups");
     p.blocks0 = (unsigned)blocks[0];
-    if (dtype == YOLO_DTYPE_BF16) hipLaunchKernelGGL(qk_norm_rope_general_kernel<true>, dim3((unsigned)total), dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(qk_norm_rope_general_kernel<false>, dim3((unsigned)total), dim3(256), 0, (hipStream_t)stream, p);
+    if (dtype == YOLO_DTYPE_BF16) launch_rope<true>(p, lpr, (unsigned)total, (hipStream_t)stream);
+    else launch_rope<false>(p, lpr, (unsigned)total, (hipStream_t)stream);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
