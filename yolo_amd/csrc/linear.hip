@@ -24,23 +24,25 @@ struct LinK {
     unsigned ntm, ntn;
 };
 
-// gelu(v) = v * Phi(v) = v/2 * erfc(-v / sqrt 2).  f32 results take the library's erfcf (no cancellation in the negative tail);
-// for bf16 results erfc(z), z >= 0, is Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7, a bf16 half step is 2^-9 of the value):
-// one reciprocal, one exponential and six multiply-adds against about forty instructions and a divergent branch, which at
-// 23104 x 4096 results cost as much time as a half of the product itself.
+// gelu(v) = v * Phi(v) = v/2 * erfc(-v / sqrt 2).  f32 results take the library's erfcf (no cancellation in the negative tail).
+// For bf16 results: max(v, 0) - |v|/2 * erfc(|v| / sqrt 2), with erfc(z) = t (a1 + t (a2 + ...)) exp(-z^2), t = 1 / (1 + 0.3275911 z),
+// Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7; a bf16 half step is 2^-9 of the value).  One reciprocal, one exponential and
+// eleven other instructions against about forty and a divergent branch: at 23104 x 4096 results the difference is a
+// quarter of the whole product's time.  The factor 1/2 is in the coefficients; |v| is cut at 16, where the exponential is 0, so that
+// +inf stays +inf.
 template <bool BF16>
 __device__ __forceinline__ float gelu(float v) {
     if constexpr (!BF16) {
         return 0.5f * v * erfcf(-0.70710678118654752f * v);
     } else {
-        const float z = __builtin_fabsf(v) * 0.70710678118654752f;
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
-        float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-        p = __builtin_fmaf(p, t, 1.421413741f);
-        p = __builtin_fmaf(p, t, -0.284496736f);
-        p = __builtin_fmaf(p, t, 0.254829592f);
-        const float e = p * t * __builtin_amdgcn_exp2f(z * z * -1.4426950408889634f);      // erfc(z)
-        return 0.5f * v * (v < 0.f ? e : 2.0f - e);
+        const float a = __builtin_fabsf(v);
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, a, 1.0f));
+        float p = __builtin_fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+        p = __builtin_fmaf(p, t, 0.5f * 1.421413741f);
+        p = __builtin_fmaf(p, t, 0.5f * -0.284496736f);
+        p = __builtin_fmaf(p, t, 0.5f * 0.254829592f);
+        const float e = p * t * __builtin_amdgcn_exp2f(v * v * -0.72134752f);      // erfc(z) / 2, log2(e) / 2
+        return __builtin_fmaf(-__builtin_fminf(a, 16.0f), e, __builtin_fmaxf(v, 0.0f));
     }
 }
 
@@ -82,14 +84,14 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     }
 }
 
-// The 16-byte piece of a row that starts at element k, elements past K as zeros.  Rows need no alignment beyond their element's:
+// The 16-byte piece at `at`, which is element k of its row, elements past K as zeros.  Rows need no alignment beyond their element's:
 // a whole piece is one load (global memory takes any address), the last one goes element by element.
 template <bool BF16>
-__device__ __forceinline__ u32x4 load_piece(const char* row, int k, int K) {
+__device__ __forceinline__ u32x4 load_piece(const char* at, int k, int K) {
     typedef typename Elem<BF16>::type T;
     constexpr int P = Elem<BF16>::kPiece;
     u32x4 v = {0, 0, 0, 0};
-    const T* p = (const T*)row + k;
+    const T* p = (const T*)at;
     if (k + P <= K) {
         __builtin_memcpy(&v, p, 16);
     } else {
@@ -103,81 +105,102 @@ __device__ __forceinline__ u32x4 load_piece(const char* row, int k, int K) {
 }
 
 // ---- tiles of BM rows of x by BN rows of W through LDS ------------------------------------------------------------------------
-// WR x WC waves, each (BM / WR) x (BN / WC); K in steps of 128 bytes, two LDS buffers, one barrier a step: the loads of step
-// s + 1 are issued before the products of step s.  An LDS row is 128 bytes = 8 pieces, piece c of row r at slot c ^ (r & 7),
-// so that the 16 rows a fragment read touches fall on all banks.  W is the MFMA's first operand: a lane then holds four
-// consecutive outputs of one row of y.
+// WR x WC waves, each (BM / WR) x (BN / WC); K in steps of 128 bytes, two LDS buffers, one barrier a step: the loads of the next
+// step are issued before the products of this one.
+// An LDS row is 128 bytes = 8 pieces, piece c of row r at slot c ^ (r & 7), so that the 16 rows a fragment read touches fall on
+// all banks.  W is the MFMA's first operand: a lane then holds four consecutive outputs of one row of y.  The accumulators start
+// from the bias.
 // ALIGNED: rows of x and W start on 16 bytes and K is whole pieces; they go global -> LDS by DMA, out-of-range rows and pieces
 // read `zero` instead.  Otherwise the pieces pass through registers.
 __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
 
+// Swaps lane rows so that a lane that holds 4 outputs of each of two 16-wide tiles (a: tile i, b: tile i + 1, packed pairs) holds 8
+// consecutive ones of one tile, and back: v_permlane16_swap is its own inverse.
+__device__ __forceinline__ void swap_pairs(uint32_t& a, uint32_t& b) {
+    const auto sw = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = sw[0];
+    b = sw[1];
+}
+
+// workgroups of a CU by LDS, at most 4
+constexpr int lin_blocks(int bm, int bn) { return bm + bn > 320 ? 1 : bm + bn > 160 ? 2 : 4; }
+
 template <bool BF16, int BM, int BN, int WR, int WC, bool ALIGNED>
-__global__ __launch_bounds__(WR* WC * 64) void linear_tile_kernel(LinK p) {
+__global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void linear_tile_kernel(LinK p) {
     typedef typename Elem<BF16>::type T;
-    constexpr int NT = WR * WC * 64, P = Elem<BF16>::kPiece, BK = 8 * P;
-    constexpr int TM = BM / WR / 16, TN = BN / WC / 16;
-    constexpr int LPT = (BM + BN) * 8 / NT;                 // pieces a thread stages per step
+    constexpr int NT = WR * WC * 64, P = Elem<BF16>::kPiece, BK = 8 * P, RPI = NT / 8;
+    constexpr int TM = BM / WR / 16, TN = BN / WC / 16, GM = 8;
+    constexpr int LX = BM / RPI, LW = BN / RPI;             // pieces of x / W a thread stages per step
     constexpr int BUF = (BM + BN) * 128;
-    static_assert((BM + BN) * 8 % NT == 0 && BM * 8 % NT == 0, "whole pieces per thread");
+    static_assert(BM % RPI == 0 && BN % RPI == 0 && RPI % 8 == 0, "whole pieces per thread");
     static_assert(TN % 2 == 0, "bf16 stores pair two column tiles");
     extern __shared__ char lds[];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const unsigned tile = xcd_chunk(blockIdx.x, p.ntm * p.ntn);
-    const unsigned tn = tile % p.ntn, tm = tile / p.ntn;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // tiles in groups of GM row tiles by all column tiles, rows first: what an XCD runs at a time is a block about as high as wide,
+    // which reads the fewest operand rows through its L2
+    const unsigned tile = xcd_chunk(blockIdx.x, p.ntm * p.ntn), group = tile / (GM * p.ntn), in = tile - group * GM * p.ntn;
+    const unsigned gm = min((unsigned)GM, p.ntm - group * GM), tn = in / gm, tm = group * GM + in - tn * gm;
     const long long m0 = (long long)tm * BM;
     const int n0 = (int)tn * BN;
     const int nsteps = (p.K + BK - 1) / BK;
+    const int fr = lane & 15, fh = lane >> 4;
+    const int wm0 = (wave / WC) * (BM / WR), wn0 = (wave % WC) * (BN / WC);
 
-    const char* src[LPT];                                   // row of piece i (nullptr: past the last row)
-    int kc;                                                 // element offset of this thread's pieces inside a step
+    // staging: this thread's piece of rows r0 + RPI i.  Rows past the last one read the last one again: their results are not stored
+    const int r0 = tid >> 3, kc = ((tid & 7) ^ (r0 & 7)) * P;
+    const int x_ld = (int)p.x_ld, w_ld = (int)p.w_ld;
+    const char *const xb = p.x + m0 * p.x_ld, *const wb = p.w + n0 * p.w_ld;
+    uint32_t off[LX + LW];
     {
-        const int r = tid >> 3;
-        kc = ((tid & 7) ^ (r & 7)) * P;                     // NT / 8 is a multiple of 8: the same for all i
+        const int mlast = (int)min((long long)BM, p.M - m0) - 1, nlast = min(BN, p.N - n0) - 1;
 #pragma unroll
-        for (int i = 0; i < LPT; ++i) {
-            const int row = i * (NT / 8) + r;
-            if (row < BM) src[i] = m0 + row < p.M ? p.x + (m0 + row) * p.x_ld : nullptr;
-            else src[i] = n0 + row - BM < p.N ? p.w + (long long)(n0 + row - BM) * p.w_ld : nullptr;
-        }
+        for (int i = 0; i < LX + LW; ++i)
+            off[i] = (uint32_t)((i < LX ? min(r0 + RPI * i, mlast) * x_ld : min(r0 + RPI * (i - LX), nlast) * w_ld) + kc * (int)sizeof(T));
     }
-    u32x4 stage[ALIGNED ? 1 : LPT];
+    u32x4 stage[ALIGNED ? 1 : LX + LW];
     auto issue = [&](int s, int buf) {
-        const int k = s * BK + kc;
+        const char *xs = xb + s * 128, *ws = wb + s * 128;
+        char* const dst = lds + buf * BUF + wave * 1024;
+        if constexpr (ALIGNED) {
+            if ((s + 1) * BK <= p.K) {
 #pragma unroll
-        for (int i = 0; i < LPT; ++i) {
-            if constexpr (ALIGNED) {
-                const bool in = src[i] != nullptr && k < p.K;
-                dma16(in ? (const void*)(src[i] + (long long)k * sizeof(T)) : (const void*)&kZeroPiece,
-                      lds + buf * BUF + (i * NT + wave * 64) * 16);
+                for (int i = 0; i < LX + LW; ++i) dma16((i < LX ? xs : ws) + off[i], dst + i * NT * 16);
             } else {
-                stage[i] = u32x4{0, 0, 0, 0};
-                if (src[i] != nullptr && k < p.K) stage[i] = load_piece<BF16>(src[i], k, p.K);
+#pragma unroll
+                for (int i = 0; i < LX + LW; ++i)
+                    dma16(s * BK + kc < p.K ? (const void*)((i < LX ? xs : ws) + off[i]) : (const void*)&kZeroPiece, dst + i * NT * 16);
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < LX + LW; ++i) stage[i] = load_piece<BF16>((i < LX ? xs : ws) + off[i], s * BK + kc, p.K);
         }
     };
     auto settle = [&](int buf) {                            // not ALIGNED: registers -> LDS
         if constexpr (!ALIGNED) {
 #pragma unroll
-            for (int i = 0; i < LPT; ++i) *(u32x4*)(lds + buf * BUF + (i * NT + tid) * 16) = stage[i];
+            for (int i = 0; i < LX + LW; ++i) *(u32x4*)(lds + buf * BUF + (i * NT + tid) * 16) = stage[i];
         }
     };
-
-    const int fr = lane & 15, fh = lane >> 4;
-    const int wm0 = (wave / WC) * (BM / WR), wn0 = (wave % WC) * (BN / WC);
     f32x4 acc[TN][TM];
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
     issue(0, 0);
+#pragma unroll
+    for (int i = 0; i < TN; ++i) {
+        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bv[r] = load_param(p.bias, p.bias_bf16, min(n0 + wn0 + i * 16 + fh * 4 + r, p.N - 1));
+        }
+#pragma unroll
+        for (int j = 0; j < TM; ++j) acc[i][j] = bv;
+    }
     settle(0);
     for (int s = 0; s < nsteps; ++s) {
+        const int buf = s & 1;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __syncthreads();
-        if (s + 1 < nsteps) issue(s + 1, (s + 1) & 1);
-        const char* bx = lds + (s & 1) * BUF;
+        if (s + 1 < nsteps) issue(s + 1, buf ^ 1);
+        const char* bx = lds + buf * BUF;
         const char* bw = bx + BM * 128;
 #pragma unroll
         for (int ks = 0; ks < 2; ++ks) {
@@ -192,89 +215,104 @@ __global__ __launch_bounds__(WR* WC * 64) void linear_tile_kernel(LinK p) {
 #pragma unroll
                 for (int j = 0; j < TM; ++j) acc[i][j] = mma<BF16>(fw[i], fx[j], acc[i][j]);
         }
-        if (s + 1 < nsteps) settle((s + 1) & 1);
+        if (s + 1 < nsteps) settle(buf ^ 1);
     }
 
     // epilogue in registers: lane holds y[m][n .. n+3] for m = wm0 + 16 j + fr, n = wn0 + 16 i + 4 fh
-    with_act(p.act, [&](auto mode) {
-        constexpr int ACT = decltype(mode)::value;
+    const bool inner = p.vec_out && m0 + BM <= p.M && n0 + BN <= p.N;
+    if (inner) {
+        // the whole tile in 16-byte pieces.  bf16: after swap_pairs a lane's piece of the tile pair i, i + 1 is 8 columns of one
+        char* const ob = p.out + m0 * p.out_ld + (long long)n0 * sizeof(T);
+        const char* const rb = p.res + m0 * p.res_ld + (long long)n0 * sizeof(T);
+        const uint32_t col = (uint32_t)(wn0 + (BF16 ? (fh & 1) * 16 + (fh >> 1) * 8 : fh * 4)) * (uint32_t)sizeof(T);
+        const uint32_t ro = (uint32_t)(wm0 + fr) * (uint32_t)p.res_ld + col, oo = (uint32_t)(wm0 + fr) * (uint32_t)p.out_ld + col;
+        // residual pieces come in two halves of the rows, the second requested before the first half's results are stored:
+        // a load behind a store would wait for it
+        constexpr int C = TM % 2 == 0 ? 2 : 1, CM = TM / C;
+        u32x4 rv[CM][TN / 2], rw[BF16 ? 1 : CM][BF16 ? 1 : TN / 2];
+        auto fetch_res = [&](int c) {
+            if (!p.res) return;
 #pragma unroll
-        for (int i = 0; i < TN; i += 2) {
-            f32x4 b0 = {0.f, 0.f, 0.f, 0.f}, b1 = {0.f, 0.f, 0.f, 0.f};
-            const int n = n0 + wn0 + i * 16 + fh * 4;
-            if (p.bias) {
+            for (int j = 0; j < CM; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (n + r < p.N) b0[r] = load_param(p.bias, p.bias_bf16, n + r);
-                    if (n + 16 + r < p.N) b1[r] = load_param(p.bias, p.bias_bf16, n + 16 + r);
+                for (int i = 0; i < TN; i += 2) {
+                    const char* q = rb + (long long)(c * CM + j) * 16 * p.res_ld + i * 16 * (int)sizeof(T) + ro;
+                    rv[j][i / 2] = *(const u32x4*)q;
+                    if constexpr (!BF16) rw[j][i / 2] = *(const u32x4*)(q + 64);
                 }
-            }
+        };
+        fetch_res(0);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            u32x4 ov[CM][TN / 2], ow[BF16 ? 1 : CM][BF16 ? 1 : TN / 2];
+            with_act(p.act, [&](auto mode) {
+                constexpr int ACT = decltype(mode)::value;
+#pragma unroll
+                for (int j = 0; j < CM; ++j)
+#pragma unroll
+                    for (int i = 0; i < TN; i += 2) {
+                        f32x4 v0, v1;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            v0[r] = activate<BF16, ACT>(acc[i][c * CM + j][r]);
+                            v1[r] = activate<BF16, ACT>(acc[i + 1][c * CM + j][r]);
+                        }
+                        if constexpr (BF16) {
+                            if (p.res) {                // brought from store order to accumulator order, added before the one rounding
+                                uint32_t q0 = rv[j][i / 2][0], q1 = rv[j][i / 2][1], q2 = rv[j][i / 2][2], q3 = rv[j][i / 2][3];
+                                swap_pairs(q0, q2);
+                                swap_pairs(q1, q3);
+                                v0 += f32x4{bf16_lo(q0), bf16_hi(q0), bf16_lo(q1), bf16_hi(q1)};
+                                v1 += f32x4{bf16_lo(q2), bf16_hi(q2), bf16_lo(q3), bf16_hi(q3)};
+                            }
+                            uint32_t a0 = pack_bf16(v0[0], v0[1]), a1 = pack_bf16(v0[2], v0[3]);
+                            uint32_t b0 = pack_bf16(v1[0], v1[1]), b1 = pack_bf16(v1[2], v1[3]);
+                            swap_pairs(a0, b0);
+                            swap_pairs(a1, b1);
+                            ov[j][i / 2] = u32x4{a0, a1, b0, b1};
+                        } else {
+                            if (p.res) {
+                                v0 += __builtin_bit_cast(f32x4, rv[j][i / 2]);
+                                v1 += __builtin_bit_cast(f32x4, rw[j][i / 2]);
+                            }
+                            ov[j][i / 2] = __builtin_bit_cast(u32x4, v0);
+                            ow[j][i / 2] = __builtin_bit_cast(u32x4, v1);
+                        }
+                    }
+            });
+            if (c + 1 < C) fetch_res(c + 1);
+#pragma unroll
+            for (int j = 0; j < CM; ++j)
+#pragma unroll
+                for (int i = 0; i < TN; i += 2) {
+                    char* o = ob + (long long)(c * CM + j) * 16 * p.out_ld + i * 16 * (int)sizeof(T) + oo;
+                    *(u32x4*)o = ov[j][i / 2];
+                    if constexpr (!BF16) *(u32x4*)(o + 64) = ow[j][i / 2];
+                }
+        }
+    } else {
+        with_act(p.act, [&](auto mode) {                // an edge, or rows off 16-byte boundaries: element by element
+            constexpr int ACT = decltype(mode)::value;
 #pragma unroll
             for (int j = 0; j < TM; ++j) {
                 const long long m = m0 + wm0 + j * 16 + fr;
-                f32x4 v0, v1;
+                if (m >= p.M) continue;
+                T* o = (T*)(p.out + m * p.out_ld);
+                const T* q = (const T*)(p.res + m * p.res_ld);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    v0[r] = activate<BF16, ACT>(acc[i][j][r] + b0[r]);
-                    v1[r] = activate<BF16, ACT>(acc[i + 1][j][r] + b1[r]);
-                }
-                if constexpr (BF16) {
-                    // v_permlane16_swap pairs the two column tiles: lane row fh then holds 8 consecutive outputs,
-                    // tile i + (fh & 1), columns 8 * (fh >> 1) .. + 7, and stores 16 bytes
-                    float o[8];
+                for (int i = 0; i < TN; ++i) {
+                    const int n = n0 + wn0 + i * 16 + fh * 4;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(v0[r]), __float_as_uint(v1[r]), false, false);
-                        o[r] = __uint_as_float(sw[0]);
-                        o[4 + r] = __uint_as_float(sw[1]);
-                    }
-                    const int nn = n0 + wn0 + (i + (fh & 1)) * 16 + (fh >> 1) * 8;
-                    if (m < p.M && nn < p.N) {
-                        char* orow = p.out + m * p.out_ld + (long long)nn * 2;
-                        const char* rrow = p.res ? p.res + m * p.res_ld + (long long)nn * 2 : nullptr;
-                        if (p.vec_out && nn + 8 <= p.N) {
-                            if (rrow) {
-                                const u32x4 rv = *(const u32x4*)rrow;
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    o[2 * q] += bf16_lo(rv[q]);
-                                    o[2 * q + 1] += bf16_hi(rv[q]);
-                                }
-                            }
-                            u32x4 ov;
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) ov[q] = pack_bf16(o[2 * q], o[2 * q + 1]);
-                            *(u32x4*)orow = ov;
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 8; ++q)
-                                if (nn + q < p.N)
-                                    ((__bf16*)orow)[q] = (__bf16)(rrow ? o[q] + (float)((const __bf16*)rrow)[q] : o[q]);
-                        }
-                    }
-                } else {
-                    if (m < p.M) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            f32x4 v = h ? v1 : v0;
-                            const int nn = n + 16 * h;
-                            if (nn >= p.N) continue;
-                            char* orow = p.out + m * p.out_ld + (long long)nn * 4;
-                            const char* rrow = p.res ? p.res + m * p.res_ld + (long long)nn * 4 : nullptr;
-                            if (p.vec_out && nn + 4 <= p.N) {
-                                if (rrow) v += *(const f32x4*)rrow;
-                                *(f32x4*)orow = v;
-                            } else {
-#pragma unroll
-                                for (int q = 0; q < 4; ++q)
-                                    if (nn + q < p.N) ((float*)orow)[q] = rrow ? v[q] + ((const float*)rrow)[q] : v[q];
-                            }
-                        }
+                        if (n + r >= p.N) continue;
+                        float v = activate<BF16, ACT>(acc[i][j][r]);
+                        if (p.res) v += load_f32(q + n + r);
+                        o[n + r] = (T)v;
                     }
                 }
             }
-        }
-    });
+        });
+    }
 }
 
 // ---- few outputs: no LDS staging, K split over the waves of a workgroup ----------------------------------------------------------
@@ -314,7 +352,7 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(LinK p) {
     auto piece = [&](const char* row, int k) {
         const bool in = row != nullptr && k < p.K;
         if constexpr (ALIGNED) return *(in ? (const u32x4*)(row + (long long)k * sizeof(T)) : &kZeroPiece);
-        else return in ? load_piece<BF16>(row, k, p.K) : u32x4{0, 0, 0, 0};
+        else return in ? load_piece<BF16>(row + (long long)k * sizeof(T), k, p.K) : u32x4{0, 0, 0, 0};
     };
     constexpr int U = 4;                                     // slices in flight; those past K read zeros
     for (int s = wave; s < nslices; s += U * W) {
@@ -389,13 +427,26 @@ static int launch_direct(LinK k, hipStream_t stream) {
     return YOLO_OK;
 }
 
+// Tile by the time of a round of tiles on the 256 CUs, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU
+// takes 4, two 128 x 128 tiles 2.4 (1060 against 1260 TFLOP/s at 8192^3, twice the operand traffic), four 64 x 64 tiles 1.7.
+// Measured (bf16, us for 256 / 128 / 64): 23104 x 4096 x 1024 220 / 246 / 316, 10816 x 512 x 1024 31.7 / 22.3 / 26.9,
+// 2704 x 1024 x 512 42 / 12.4 / 9.6; f32 has no 256 x 256 (288 against 216 at 23104 x 1024 x 512: its registers do not fit).
+// Few outputs go to the direct kernel, which splits K inside a workgroup: up to 512 tiles of 16 x 16 (40 x 1024 x 1024: 4.1 against 6.7 in
+// 32 x 32 and 8.2 in 64 x 64), up to 256 of 32 x 32 (300 x 512 x 1024: 7.4 against 11.2; 700 x 512 x 512, 352 tiles: 9.0 against 7.9).
+// The direct kernel forms 64-bit addresses; the tile kernel offsets rows of a tile in 32 bits and takes strides up to 4 MB.
 template <bool BF16>
 static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
-    const unsigned long long t128 = (unsigned long long)((k.M + 127) / 128) * ((k.N + 127) / 128);
-    if (k.M <= 16) return aligned ? launch_direct<BF16, 1, 1, true>(k, stream) : launch_direct<BF16, 1, 1, false>(k, stream);
-    if (t128 < 64) return aligned ? launch_direct<BF16, 2, 2, true>(k, stream) : launch_direct<BF16, 2, 2, false>(k, stream);
-    if (aligned) return launch_tile<BF16, 128, 128, 2, 2, true>(k, stream);
-    return launch_tile<BF16, 128, 128, 2, 2, false>(k, stream);
+    auto tiles = [&](int e) { return (unsigned long long)((k.M + e - 1) / e) * ((k.N + e - 1) / e); };
+    const long long kMaxStride = 1ll << 22;
+    const bool wide = k.x_ld > kMaxStride || k.w_ld > kMaxStride || k.out_ld > kMaxStride || (k.res && k.res_ld > kMaxStride);
+    if (tiles(16) <= 512) return aligned ? launch_direct<BF16, 1, 1, true>(k, stream) : launch_direct<BF16, 1, 1, false>(k, stream);
+    if (tiles(32) <= 256 || wide) return aligned ? launch_direct<BF16, 2, 2, true>(k, stream) : launch_direct<BF16, 2, 2, false>(k, stream);
+    const double c256 = (double)((tiles(256) + 255) / 256) * 4.0, c128 = (double)((tiles(128) + 511) / 512) * 2.4, c64 = (double)((tiles(64) + 1023) / 1024) * 1.7;
+    if constexpr (BF16) {
+        if (aligned && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
+    }
+    if (c128 <= c64) return aligned ? launch_tile<BF16, 128, 128, 2, 2, true>(k, stream) : launch_tile<BF16, 128, 128, 2, 2, false>(k, stream);
+    return aligned ? launch_tile<BF16, 64, 64, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 2, 2, false>(k, stream);
 }
 
 }  // namespace yolo
