@@ -24,7 +24,8 @@ def empty(shape, dtype=torch.float32):
 
 
 def stream_ptr():
-    return torch.cuda.current_stream().cuda_stream
+    """hipStream_t of the current stream: torch.cuda.current_stream().cuda_stream without building a Stream object (0.1 us for 2.7)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def ptr(t):

@@ -148,8 +148,11 @@ _DTYPE_CODES = {torch.float32: _lib.YOLO_DTYPE_F32, torch.bfloat16: _lib.YOLO_DT
 _ACTIVATIONS = {None: 0, "linear": 0, "leaky": 1, "relu": 2, "gelu": 3, "silu": 4}
 
 
-def _dev(x, name, dtype=None):
-    """numpy / torch (any device) -> tensor of its own type (or `dtype`) on the current GPU, strides kept."""
+_Strides = ctypes.c_int64 * 3
+
+
+def _dev(x, name, dev, dtype=None):
+    """numpy / torch (any device) -> tensor of its own type (or `dtype`) on the current GPU `dev`, strides kept."""
     if not isinstance(x, torch.Tensor):
         x = torch.from_numpy(np.asarray(x))
         if x.dtype == torch.float64 and dtype is None:
@@ -158,7 +161,7 @@ def _dev(x, name, dtype=None):
         raise ValueError("%s requires a gradient: yolo_amd implements the inference path only (call under torch.no_grad())" % name)
     if dtype is not None and x.dtype != dtype:
         x = x.to(dtype)
-    if not x.is_cuda or x.get_device() != torch.cuda.current_device():
+    if x.get_device() != dev:
         x = x.to(_tensor.device())
     return x
 
@@ -176,14 +179,21 @@ def _same_type(x, like, name):
     return x
 
 
-def _param(x, n, name):
+def _param(x, n, name, dev):
     """Bias / norm weight: [n] contiguous, float32 or bfloat16 -> (tensor or None, type code)."""
     if x is None:
         return None, 0
-    x = _dev(x, name)
-    if x.dim() != 1 or x.shape[0] != n:
+    x = _dev(x, name, dev)
+    if x.shape != (n,):
         raise ValueError("%s must be [%d], got %s" % (name, n, tuple(x.shape)))
     return x.contiguous(), _code(x, name)
+
+
+def _gpu():
+    """Index of the current GPU; like `_tensor.device()` an error without one."""
+    if not torch.cuda.is_initialized():
+        _tensor.device()
+    return torch.cuda.current_device()
 
 
 def _rows(x):
@@ -212,23 +222,24 @@ def linear(inputs, weight, bias=None, activation=None, residual=None):
     """act(inputs @ weight.T + bias) + residual in one launch: inputs [..., K] (a map's cells [B, H, W, K] as they are), weight
     [N, K], bias [N], residual [..., N] -> [..., N], float32 or bfloat16 throughout (bias: either).  activation: None, "leaky"
     (slope 0.1), "relu", "gelu" (error function) or "silu"; the residual is added after it, as in res_block.  yolo_linear."""
-    x, w = _dev(inputs, "inputs"), _dev(weight, "weight")
+    dev = _gpu()
+    x, w = _dev(inputs, "inputs", dev), _dev(weight, "weight", dev)
     code = _code(x, "inputs")
     _same_type(w, x, "weight")
     if activation not in _ACTIVATIONS:
         raise ValueError("linear: unknown activation %r" % (activation,))
     if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.shape[1] == 0 or w.shape[0] == 0:
         raise ValueError("linear: inputs %s do not fit weight %s" % (tuple(x.shape), tuple(w.shape)))
-    N, K = int(w.shape[0]), int(w.shape[1])
-    b, bcode = _param(bias, N, "bias")
+    N, K = w.shape
+    b, bcode = _param(bias, N, "bias", dev)
     shape = x.shape[:-1] + (N,)
     r, r_ld = None, 0
     if residual is not None:
-        r = _same_type(_dev(residual, "residual"), x, "residual")
+        r = _same_type(_dev(residual, "residual", dev), x, "residual")
         if r.shape != shape:
             raise ValueError("linear: residual %s, expected %s" % (tuple(r.shape), tuple(shape)))
         r, r_ld = _rows(r)
-    out = torch.empty(shape, dtype=x.dtype, device=x.device)
+    out = x.new_empty(shape)
     M = out.numel() // N
     x, x_ld = _rows(x)
     w, w_ld = _rows(w)
@@ -255,12 +266,12 @@ def _heads(x, name):
     if st[3] != 1 and x.shape[3] > 1:
         x = x.contiguous()
         st = x.stride()
-    return x, (ctypes.c_int64 * 3)(st[0], st[1], st[2])
+    return x, _Strides(st[0], st[1], st[2])
 
 
-def _positions(p, B, L, axes, name):
+def _positions(p, B, L, axes, name, dev):
     """-> (contiguous tensor, batched).  [L] / [B, L] for one axis, [L, 2] / [B, L, 2] for two; a trailing 1 is allowed for one."""
-    p = _dev(p, name)
+    p = _dev(p, name, dev)
     if p.dtype not in (torch.int32, torch.int64):
         raise ValueError("%s must be int32 or int64, got %s" % (name, p.dtype))
     shape = tuple(p.shape)
@@ -281,43 +292,44 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, frequencies=None, q_positio
     column), where the first half of the pairs turns by the row and the second by the column.  `axes` (1 or 2) says which where
     None would leave [B, L] = [L, 2] open.  Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) if `interleaved`.
     yolo_qk_norm_rope."""
-    q, qs = _heads(_dev(q, "q"), "q")
+    dev = _gpu()
+    q, qs = _heads(_dev(q, "q", dev), "q")
     code = _code(q, "q")
-    B, Lq, Hq, D = [int(v) for v in q.shape]
+    B, Lq, Hq, D = q.shape
     Lk, Hk, ks, ko = 0, 0, None, None
     if k is not None:
-        k, ks = _heads(_same_type(_dev(k, "k"), q, "k"), "k")
-        Lk, Hk = int(k.shape[1]), int(k.shape[2])
+        k, ks = _heads(_same_type(_dev(k, "k", dev), q, "k"), "k")
+        Lk, Hk = k.shape[1:3]
         if k.shape[0] != B or k.shape[3] != D:
             raise ValueError("qk_norm_rope: k %s does not fit q %s" % (tuple(k.shape), tuple(q.shape)))
-        ko = torch.empty((B, Lk, Hk, D), dtype=q.dtype, device=q.device)
-    qw, qwc = _param(q_weight, D, "q_weight")
-    kw, kwc = _param(k_weight if k is not None else None, D, "k_weight")
+        ko = q.new_empty((B, Lk, Hk, D))
+    qw, qwc = _param(q_weight, D, "q_weight", dev)
+    kw, kwc = _param(k_weight if k is not None else None, D, "k_weight", dev)
     if qw is not None and kw is not None and qwc != kwc:
         raise ValueError("q_weight and k_weight must be of one type")
     qp = kp = None
     R, pos64, qb, kb = 0, 0, 0, 0
     if frequencies is not None:
-        frequencies = _dev(frequencies, "frequencies", torch.float64).contiguous()
+        frequencies = _dev(frequencies, "frequencies", dev, torch.float64).contiguous()
         if frequencies.dim() != 1 or not 0 < 2 * frequencies.shape[0] <= D:
             raise ValueError("qk_norm_rope: frequencies %s for heads of %d" % (tuple(frequencies.shape), D))
         R = 2 * int(frequencies.shape[0])
         if q_positions is None or (k is not None and k_positions is None):
             raise ValueError("qk_norm_rope: frequencies need positions")
-        q_positions = _dev(q_positions, "q_positions")
+        q_positions = _dev(q_positions, "q_positions", dev)
         if axes is None:
             if tuple(q_positions.shape) == (2, 2) == (B, Lq):
                 raise ValueError("qk_norm_rope: positions [2, 2] of 2 x 2 queries may be one axis or two: pass axes")
             axes = 2 if q_positions.dim() > 1 and q_positions.shape[-1] == 2 and tuple(q_positions.shape) != (B, Lq) else 1
         if axes not in (1, 2) or R // 2 % axes:
             raise ValueError("qk_norm_rope: %d pairs over %r axes" % (R // 2, axes))
-        qp, qb = _positions(q_positions, B, Lq, axes, "q_positions")
+        qp, qb = _positions(q_positions, B, Lq, axes, "q_positions", dev)
         if k is not None:
-            kp, kb = _positions(k_positions, B, Lk, axes, "k_positions")
+            kp, kb = _positions(k_positions, B, Lk, axes, "k_positions", dev)
             if kp.dtype != qp.dtype:
                 kp, qp = kp.long(), qp.long()
         pos64 = int(qp.dtype == torch.int64)
-    qo = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    qo = q.new_empty((B, Lq, Hq, D))
     if D == 0 or Hq == 0 or (k is not None and Hk == 0):
         raise ValueError("qk_norm_rope: no heads in q %s" % (tuple(q.shape),))
     _lib.check(_lib.lib().yolo_qk_norm_rope(
@@ -333,32 +345,33 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     h // (Hq // Hk).  key_lens [B] int32: keys from key_lens[b] on are padding; key_mask [B, Lk] bool: False leaves a key out.
     What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.
     -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
-    q, qs = _heads(_dev(q, "q"), "q")
+    dev = _gpu()
+    q, qs = _heads(_dev(q, "q", dev), "q")
     code = _code(q, "q")
-    k, ks = _heads(_same_type(_dev(k, "k"), q, "k"), "k")
-    v, vs = _heads(_same_type(_dev(v, "v"), q, "v"), "v")
-    B, Lq, Hq, D = [int(n) for n in q.shape]
-    Lk, Hk = int(k.shape[1]), int(k.shape[2])
+    k, ks = _heads(_same_type(_dev(k, "k", dev), q, "k"), "k")
+    v, vs = _heads(_same_type(_dev(v, "v", dev), q, "v"), "v")
+    B, Lq, Hq, D = q.shape
+    Lk, Hk = k.shape[1:3]
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
         raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError("cross_attention: %d query heads over %d key heads of %d" % (Hq, Hk, D))
     if key_lens is not None:
-        key_lens = _dev(key_lens, "key_lens")
+        key_lens = _dev(key_lens, "key_lens", dev)
         if tuple(key_lens.shape) != (B,) or key_lens.dtype not in (torch.int32, torch.int64):
             raise ValueError("key_lens must be int32 [%d], got %s %s" % (B, key_lens.dtype, tuple(key_lens.shape)))
         if key_lens.dtype == torch.int64:
             key_lens = key_lens.clamp(0, Lk).to(torch.int32)
         key_lens = key_lens.contiguous()
     if key_mask is not None:
-        key_mask = _dev(key_mask, "key_mask")
+        key_mask = _dev(key_mask, "key_mask", dev)
         if tuple(key_mask.shape) != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8):
             raise ValueError("key_mask must be bool [%d, %d], got %s %s" % (B, Lk, key_mask.dtype, tuple(key_mask.shape)))
         key_mask = key_mask.contiguous()
-    out = torch.empty((B, Lq, Hq, D), dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, Lq, Hq, D))
     L = _lib.lib()
     need = L.yolo_cross_attention_workspace_bytes(code, B, Lq, Lk, Hq, Hk, D)
-    ws = _tensor.workspace(need) if need else None
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _lib.check(L.yolo_cross_attention(code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _tensor.ptr(key_lens),
                                       _tensor.ptr(key_mask), B, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None else float(scale),
                                       out.data_ptr(), _tensor.ptr(ws), need, _tensor.stream_ptr()))
