@@ -130,7 +130,7 @@ __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
 template <bool BF16, int DC> struct AttnTile {
     static constexpr int Z = BF16 ? 2 : 4, P = 16 / Z;                              // bytes and elements of a piece
     static constexpr int ROW = DC * Z <= 64 ? 64 : DC * Z <= 128 ? 128 : DC * Z <= 256 ? 256 : DC * Z <= 512 ? 512 : 1024;
-    static constexpr int PCS = ROW / 16, KT = ROW > 512 ? 32 : 64;                  // pieces of an LDS row, keys per tile
+    static constexpr int PCS = ROW / 16, KT = ROW >= 512 ? 32 : 64;                  // pieces of an LDS row, keys per tile
     static constexpr int RPL = ROW >= 256 ? 1 : 256 / ROW;                          // rows per 256 bytes (all banks)
     static constexpr int TILE = KT * ROW;                                           // bytes of one k or v tile
     static constexpr int LDS = 4 * TILE;
@@ -144,8 +144,8 @@ template <bool BF16, int DC> struct AttnTile {
     }
 };
 
-template <bool BF16, int DC, int WAVES, int NQ>
-__global__ __launch_bounds__(WAVES * 64) void cross_attention_tile_kernel(AttnK p) {
+template <bool BF16, int DC, int WAVES, int NQ, int MW>
+__global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(AttnK p) {
     typedef typename Elem<BF16>::type T;
     typedef AttnTile<BF16, DC> L;
     constexpr int P = L::P, PCS = L::PCS, KT = L::KT, NT = WAVES * 64;
@@ -224,21 +224,24 @@ __global__ __launch_bounds__(WAVES * 64) void cross_attention_tile_kernel(AttnK 
         char* vd = lds + (2 + buf) * L::TILE + wave * 1024;
         const char* ks = kbase + ((long long)t * KT + r0) * kls;
         const char* vs = vbase + ((long long)t * KT + r0) * vls;
-        const bool plain = !padded && (kept & full) == full;
+        auto each_piece = [&](auto plain) {
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const int r = r0 + i * RPI;
-            const int kc = L::kpiece(r, slot), vc = L::vpiece(r, slot);
-            const char* kg = ks + (long long)(i * RPI) * kls + kc * 16;
-            const char* vg = vs + (long long)(i * RPI) * vls + vc * 16;
-            if (!plain) {
-                const bool in = (kept >> r) & 1;
-                if (!in || kc * P >= p.D) kg = (const char*)&kZeroPiece;
-                if (!in || vc * P >= p.D) vg = (const char*)&kZeroPiece;
+            for (int i = 0; i < NI; ++i) {
+                const int r = r0 + i * RPI;
+                const int kc = L::kpiece(r, slot), vc = L::vpiece(r, slot);
+                const char* kg = ks + (long long)(i * RPI) * kls + kc * 16;
+                const char* vg = vs + (long long)(i * RPI) * vls + vc * 16;
+                if constexpr (!plain.value) {
+                    const bool in = (kept >> r) & 1;
+                    kg = in && kc * P < p.D ? kg : (const char*)&kZeroPiece;
+                    vg = in && vc * P < p.D ? vg : (const char*)&kZeroPiece;
+                }
+                dma16(kg, kd + i * NT * 16);
+                dma16(vg, vd + i * NT * 16);
             }
-            dma16(kg, kd + i * NT * 16);
-            dma16(vg, vd + i * NT * 16);
-        }
+        };
+        if (!padded && (kept & full) == full) each_piece(std::true_type{});
+        else each_piece(std::false_type{});
     };
 
     bool any = false;
@@ -413,17 +416,18 @@ __global__ __launch_bounds__(WAVES * 64) void cross_attention_tile_kernel(AttnK 
     }
 }
 
-// Joins the key splits of a row: one wave per row, lane = split for the maxima and sums, lane + 64 i = element for the results.
-// The splits are added in order: the result does not depend on the launch.
+// Joins the key splits of a row: WPR waves per row, lane = split for the maxima and sums, lane + 64 i = element for the results; a
+// wave adds every WPR-th split with four loads in flight, the waves' sums are added in order: the result does not depend on the launch.
 constexpr int kMaxSplits = 64;
 
-template <bool BF16>
+template <bool BF16, int WPR>
 __global__ __launch_bounds__(256) void cross_attention_join_kernel(AttnK p) {
     typedef typename Elem<BF16>::type T;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ float sums[WPR > 1 ? WPR : 1][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w0 = wave % WPR;
     const long long total = (long long)p.B * p.Lq * p.Hq;
-    const long long row = (long long)blockIdx.x * 4 + wave;
-    if (row >= total) return;
+    const long long row = (long long)blockIdx.x * (4 / WPR) + wave / WPR;
+    if (row >= total) return;                               // WPR = 4: the whole workgroup
     const bool have = lane < p.splits;
     const float2 ml = have ? p.ml[lane * total + row] : make_float2(-__builtin_inff(), -1.0f);
     const bool kept = have && ml.y != -1.0f;                // a NaN sum is kept
@@ -431,20 +435,37 @@ __global__ __launch_bounds__(256) void cross_attention_join_kernel(AttnK p) {
     float m = kept ? ml.x : -__builtin_inff();
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    // a split whose kept scores are all -inf has maximum -inf, sum 0 and results 0
-    float w = kept && ml.x != -__builtin_inff() ? __builtin_amdgcn_exp2f((ml.x - m) * p.scale2) : kept && ml.y == 0.f ? 0.f : kept ? 1.f : 0.f;
+    // a split without a kept key has results 0; one whose kept scores are all -inf has maximum -inf, sum 0 and results 0, or a NaN sum
+    const float w = !kept ? 0.f : ml.x != -__builtin_inff() ? __builtin_amdgcn_exp2f((ml.x - m) * p.scale2) : ml.y == 0.f ? 0.f : 1.f;
     float l = kept ? w * ml.y : 0.f;
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
     float o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < p.splits; ++s) {
-        const float ws = __shfl(w, s);
-        if (!__shfl((int)kept, s)) continue;
+    for (int s0 = w0; s0 < p.splits; s0 += 4 * WPR) {
+        float v[4][4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int d = lane + 64 * i;
-            if (d < p.D) o[i] = __builtin_fmaf(ws, p.part[(s * total + row) * p.D + d], o[i]);
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int s = s0 + u * WPR, d = lane + 64 * i;
+                v[u][i] = s < p.splits && d < p.D ? p.part[(s * total + row) * p.D + d] : 0.f;
+            }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float ws = __shfl(w, (s0 + u * WPR) & 63);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(ws, v[u][i], o[i]);
         }
+    }
+    if constexpr (WPR > 1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[w0][lane + 64 * i] = o[i];
+        __syncthreads();
+        if (w0) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 1; x < WPR; ++x) o[i] += sums[x][lane + 64 * i];
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -459,30 +480,49 @@ struct AttnPlan {
     size_t bytes;
 };
 
+// The number of key splits S is the one of least modelled time, in microseconds: rounds of workgroups times the tiles of one, and for
+// S > 1 the join's launch and the traffic of the partial results.  Measured (bf16, us at S = 1 / 2 / 4): 32 x 100 queries of 8 heads of 64 over
+// 3549 keys 74 / 65 / 68, 16 x 100 of 128 over 3549 101 / 69 / 64, 64 x 2704 of 64 over 80 keys 133 / 710 / 710; one query of 16
+// heads over 3549 keys 54 at S = 1, 11 at 56.  Eight waves share a tile's loads where their larger row tiles still fill the CUs as
+// well (8 x 2704 queries of 8 heads of 128: 524 against 553), not over few tiles (80 keys, above: 153).
 static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
     AttnPlan a;
-    const int z = dtype == YOLO_DTYPE_BF16 ? 2 : 4;
+    const bool bf16 = dtype == YOLO_DTYPE_BF16;
     a.dc = D <= 32 ? 32 : D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256;
-    a.kt = a.dc * z > 512 ? 32 : 64;
-    const long long rows = (long long)Lq * (Hq / Hk);
-    a.waves = rows <= 32 ? 1 : 4;
+    a.kt = a.dc * (bf16 ? 2 : 4) > 256 ? 32 : 64;
+    const long long rows = (long long)Lq * (Hq / Hk), groups = (long long)B * Hk;
+    auto rtiles = [&](int waves) { return (rows + 32 * waves - 1) / (32 * waves); };
+    auto rounds = [](long long blocks, long long slots) { return (blocks + slots - 1) / slots; };
+    a.waves = rows <= 32 && a.dc < 256 ? 1 : 4;
     a.nq = 1;
-    a.rtiles = (int)((rows + 32 * a.waves * a.nq - 1) / (32 * a.waves * a.nq));
-    const long long blocks = (long long)a.rtiles * B * Hk;
     const int tiles = (Lk + a.kt - 1) / a.kt;
-    // few row tiles: the keys are split until there are about 512 workgroups (1024 of one wave)
-    const long long want = a.waves == 1 ? 1024 : 512;
-    long long s = blocks >= want / 2 ? 1 : want / blocks;
-    if (s > tiles) s = tiles;
-    if (s > kMaxSplits) s = kMaxSplits;
-    if (s < 1) s = 1;
-    a.tps = tiles ? (int)((tiles + s - 1) / s) : 0;
-    a.splits = a.tps ? (tiles + a.tps - 1) / a.tps : 1;
+    if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) a.waves = 8;
+    a.rtiles = (int)rtiles(a.waves);
+    const long long blocks = a.rtiles * groups;
+    // workgroups at a time: by registers and LDS two of four waves to a CU in bf16, one where a wave has the whole register file
+    // or, in f32, the matrix cores are busy with one
+    const long long slots = a.waves == 1 ? 1024 : a.waves == 4 && bf16 && a.dc < 256 ? 512 : 256;
+    const double tile_us = bf16 ? 0.4 + 0.6 * a.dc / 128 * a.kt / 64 : 3.5 * a.dc / 64 * a.kt / 64;
+    const double join_us = 4e-6 * 2 * B * Lq * (double)Hq * D / 4;                  // of one more split, at 4 TB/s
+    double best = 0;
+    a.splits = 1;
+    a.tps = tiles;
+    for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
+        const int tps = (tiles + s - 1) / s, splits = (tiles + tps - 1) / tps;
+        const double t = (double)rounds(blocks * splits, slots) * (tps + 1) * tile_us + (splits > 1 ? 4.0 + splits * (0.04 + join_us) : 0.0);
+        if (s == 1 || t < best) {
+            best = t;
+            a.splits = splits;
+            a.tps = tps;
+        }
+    }
     a.bytes = a.splits > 1 ? (size_t)a.splits * B * Lq * Hq * (D + 2) * 4 : 0;
     return a;
 }
 
-template <bool BF16, int DC, int WAVES, int NQ>
+// MW: waves per SIMD the register budget is cut for.  Two hide each other's latencies where the tiles fill the GPU (D = 128, four waves:
+// 804 us at one, 553 at two); one-wave workgroups run one to a SIMD, and 256 elements of o, q and their tiles need all 512 registers
+template <bool BF16, int DC, int WAVES, int NQ, int MW = (WAVES == 1 || DC == 256 || (!BF16 && DC > 64)) ? 1 : 2>
 static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
     constexpr int kLds = AttnTile<BF16, DC>::LDS;
     if (kLds > 64 * 1024) {
@@ -490,21 +530,26 @@ static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
         int dev = 0;
         YOLO_HIP_CHECK(hipGetDevice(&dev));
         if (dev >= 16 || !attr_done[dev]) {
-            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, NQ>,
+            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, NQ, MW>,
                                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
             if (dev < 16) attr_done[dev] = true;
         }
     }
     const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk;
     YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 workgroups");
-    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, NQ>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
+    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, NQ, MW>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
 
 template <bool BF16, int DC>
 static int launch_attn_dc(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
-    if (a.waves == 1) return launch_attn_tile<BF16, DC, 1, 1>(p, stream);
+    if constexpr (BF16 && (DC == 64 || DC == 96 || DC == 128)) {
+        if (a.waves == 8) return launch_attn_tile<BF16, DC, 8, 1>(p, stream);
+    }
+    if constexpr (DC < 256) {
+        if (a.waves == 1) return launch_attn_tile<BF16, DC, 1, 1>(p, stream);
+    }
     return launch_attn_tile<BF16, DC, 4, 1>(p, stream);
 }
 
@@ -519,9 +564,11 @@ static int launch_attn(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
         default: rc = launch_attn_dc<BF16, 256>(p, a, stream); break;
     }
     if (rc != YOLO_OK || p.splits == 1) return rc;
-    const unsigned long long blocks = ((unsigned long long)p.B * p.Lq * p.Hq + 3) / 4;
-    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^33 rows");
-    hipLaunchKernelGGL(cross_attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    // four waves per row where a row has more than one batch of loads
+    const unsigned long long rows = (unsigned long long)p.B * p.Lq * p.Hq, blocks = p.splits > 4 ? rows : (rows + 3) / 4;
+    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 rows");
+    if (p.splits > 4) hipLaunchKernelGGL((cross_attention_join_kernel<BF16, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((cross_attention_join_kernel<BF16, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
