@@ -191,9 +191,11 @@ def _param(x, n, name, dev):
 
 def _gpu():
     """Index of the current GPU; like `_tensor.device()` an error without one."""
-    if not torch.cuda.is_initialized():
+    try:
+        return torch.cuda.current_device()
+    except Exception:
         _tensor.device()
-    return torch.cuda.current_device()
+        raise
 
 
 def _rows(x):
@@ -226,25 +228,26 @@ def linear(inputs, weight, bias=None, activation=None, residual=None):
     x, w = _dev(inputs, "inputs", dev), _dev(weight, "weight", dev)
     code = _code(x, "inputs")
     _same_type(w, x, "weight")
-    if activation not in _ACTIVATIONS:
+    act = _ACTIVATIONS.get(activation, -1)
+    if act < 0:
         raise ValueError("linear: unknown activation %r" % (activation,))
-    if x.dim() < 1 or w.dim() != 2 or w.shape[1] != x.shape[-1] or w.shape[1] == 0 or w.shape[0] == 0:
-        raise ValueError("linear: inputs %s do not fit weight %s" % (tuple(x.shape), tuple(w.shape)))
-    N, K = w.shape
+    shape, wshape = tuple(x.shape), w.shape
+    if not shape or len(wshape) != 2 or wshape[1] != shape[-1] or wshape[1] == 0 or wshape[0] == 0:
+        raise ValueError("linear: inputs %s do not fit weight %s" % (shape, tuple(wshape)))
+    N, K = wshape
     b, bcode = _param(bias, N, "bias", dev)
-    shape = x.shape[:-1] + (N,)
+    shape = shape[:-1] + (N,)
     r, r_ld = None, 0
     if residual is not None:
         r = _same_type(_dev(residual, "residual", dev), x, "residual")
         if r.shape != shape:
-            raise ValueError("linear: residual %s, expected %s" % (tuple(r.shape), tuple(shape)))
+            raise ValueError("linear: residual %s, expected %s" % (tuple(r.shape), shape))
         r, r_ld = _rows(r)
     out = x.new_empty(shape)
-    M = out.numel() // N
     x, x_ld = _rows(x)
     w, w_ld = _rows(w)
     _lib.check(_lib.lib().yolo_linear(code, x.data_ptr(), x_ld, w.data_ptr(), w_ld, _tensor.ptr(b), bcode, _tensor.ptr(r), r_ld,
-                                      out.data_ptr(), N, M, N, K, _ACTIVATIONS[activation], _tensor.stream_ptr()))
+                                      out.data_ptr(), N, out.numel() // N, N, K, act, _tensor.stream_ptr(dev)))
     return out
 
 
@@ -335,7 +338,7 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, frequencies=None, q_positio
     _lib.check(_lib.lib().yolo_qk_norm_rope(
         code, B, D, q.data_ptr(), qs, Lq, Hq, _tensor.ptr(qw), _tensor.ptr(qp), qo.data_ptr(),
         _tensor.ptr(k), ks, Lk, Hk, _tensor.ptr(kw), _tensor.ptr(kp), _tensor.ptr(ko), qwc if qw is not None else kwc,
-        _tensor.ptr(frequencies), R, axes or 1, pos64, qb, kb, int(bool(interleaved)), float(eps), _tensor.stream_ptr()))
+        _tensor.ptr(frequencies), R, axes or 1, pos64, qb, kb, int(bool(interleaved)), float(eps), _tensor.stream_ptr(dev)))
     return qo, ko
 
 
@@ -374,5 +377,5 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _lib.check(L.yolo_cross_attention(code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _tensor.ptr(key_lens),
                                       _tensor.ptr(key_mask), B, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None else float(scale),
-                                      out.data_ptr(), _tensor.ptr(ws), need, _tensor.stream_ptr()))
+                                      out.data_ptr(), _tensor.ptr(ws), need, _tensor.stream_ptr(dev)))
     return out
