@@ -525,3 +525,24 @@ def test_refusals(L):
             pytest.fail("call %d was accepted" % i)
     with torch.no_grad():
         assert torch.equal(L.linear(x, w.clone().requires_grad_()), L.linear(x, w))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d", [(1, 1, 40000, 4, 4, 64), (1, 2, 33333, 8, 2, 128), (2, 40, 20001, 2, 1, 64), (1, 1, 9000, 2, 2, 256), (3, 1, 15000, 2, 1, 32)])
+def test_attention_long_states(L, t, b, lq, lk, hq, hk, d):
+    """Few queries over long states: the keys are split over workgroups and joined."""
+    q, k, v = qkv(t, b, lq, lk, hq, hk, d, 95)
+    check_attention(L, q, k, v)
+    lens = torch.tensor([lk - 7, 0, lk // 3][:b], dtype=torch.int32, device="cuda")
+    check_attention(L, q, k, v, lens=lens, what=("lens",))
+    k[:, lk // 2:, 0, 0] = float("nan")
+    keep = torch.ones((b, lk), dtype=torch.bool, device="cuda")
+    keep[:, lk // 2:] = False
+    keep[:, 3] = False
+    v[:, 3] = float("inf")
+    check_attention(L, q, k, v, lens=lens, mask=keep, what=("both",))
+    k[:, 5, 0, 0] = float("nan")
+    got = L.cross_attention(q, k, v, key_mask=keep)
+    assert got[:, :, :hq // hk].isnan().all()
+    if hk > 1:
+        assert torch.isfinite(got[:, :, hq // hk:]).all()

@@ -483,7 +483,7 @@ struct AttnPlan {
 // The number of key splits S is the one of least modelled time, in microseconds: rounds of workgroups times the tiles of one, and for
 // S > 1 the join's launch and the traffic of the partial results.  Measured (bf16, us at S = 1 / 2 / 4): 32 x 100 queries of 8 heads of 64 over
 // 3549 keys 74 / 65 / 68, 16 x 100 of 128 over 3549 101 / 69 / 64, 64 x 2704 of 64 over 80 keys 133 / 710 / 710; one query of 16
-// heads over 3549 keys 54 at S = 1, 11 at 56.  Eight waves share a tile's loads where their larger row tiles still fill the CUs as
+// heads of 64, 4 key heads: 9.1 at S = 1, 8.5 at 5 over 300 keys; 28 at 1, 8.9 at 12 over 1444; 64 at 1, 10 at 28 over 3549.  Eight waves share a tile's loads where their larger row tiles still fill the CUs as
 // well (8 x 2704 queries of 8 heads of 128: 524 against 553), not over few tiles (80 keys, above: 153).
 static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
     AttnPlan a;
@@ -502,14 +502,16 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     // workgroups at a time: by registers and LDS two of four waves to a CU in bf16, one where a wave has the whole register file
     // or, in f32, the matrix cores are busy with one
     const long long slots = a.waves == 1 ? 1024 : a.waves == 4 && bf16 && a.dc < 256 ? 512 : 256;
-    const double tile_us = bf16 ? 0.4 + 0.6 * a.dc / 128 * a.kt / 64 : 3.5 * a.dc / 64 * a.kt / 64;
+    // a one-wave workgroup alone on its SIMD: 1.07 us a tile (64 of 64, bf16), its loads' latency
+    const double tile_us = (bf16 ? 0.4 + 0.6 * a.dc / 128 * a.kt / 64 : 3.5 * a.dc / 64 * a.kt / 64) * (a.waves == 1 ? 1.5 : 1.0);
+    const double join_fixed_us = a.waves == 1 ? 7.0 : 4.0;                          // where latency counts also the launch on the host
     const double join_us = 4e-6 * 2 * B * Lq * (double)Hq * D / 4;                  // of one more split, at 4 TB/s
     double best = 0;
     a.splits = 1;
     a.tps = tiles;
     for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
         const int tps = (tiles + s - 1) / s, splits = (tiles + tps - 1) / tps;
-        const double t = (double)rounds(blocks * splits, slots) * (tps + 1) * tile_us + (splits > 1 ? 4.0 + splits * (0.04 + join_us) : 0.0);
+        const double t = (double)rounds(blocks * splits, slots) * (tps + 1) * tile_us + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
         if (s == 1 || t < best) {
             best = t;
             a.splits = splits;
