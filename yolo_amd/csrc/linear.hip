@@ -20,7 +20,6 @@ struct LinK {
     long long M;
     int N, K;
     int bias_bf16, act;
-    int vec_out;                            // out / residual rows are 16-byte aligned
     unsigned ntm, ntn;
 };
 
@@ -218,14 +217,17 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
         if (s + 1 < nsteps) settle(buf ^ 1);
     }
 
-    // epilogue in registers: lane holds y[m][n .. n+3] for m = wm0 + 16 j + fr, n = wn0 + 16 i + 4 fh
-    const bool inner = p.vec_out && m0 + BM <= p.M && n0 + BN <= p.N;
-    if (inner) {
-        // the whole tile in 16-byte pieces.  bf16: after swap_pairs a lane's piece of the tile pair i, i + 1 is 8 columns of one
-        char* const ob = p.out + m0 * p.out_ld + (long long)n0 * sizeof(T);
-        const char* const rb = p.res + m0 * p.res_ld + (long long)n0 * sizeof(T);
-        const uint32_t col = (uint32_t)(wn0 + (BF16 ? (fh & 1) * 16 + (fh >> 1) * 8 : fh * 4)) * (uint32_t)sizeof(T);
-        const uint32_t ro = (uint32_t)(wm0 + fr) * (uint32_t)p.res_ld + col, oo = (uint32_t)(wm0 + fr) * (uint32_t)p.out_ld + col;
+    // epilogue in registers: lane holds y[m][n .. n+3] for m = wm0 + 16 j + fr, n = wn0 + 16 i + 4 fh.  Results leave and residuals come in
+    // pieces of 16 bytes wherever their rows start (global memory takes any address).  bf16: after swap_pairs a lane's piece of the
+    // tile pair i, i + 1 is 8 columns of one of the two; f32: 4 columns of each.
+    char* const ob = p.out + m0 * p.out_ld + (long long)n0 * sizeof(T);
+    const char* const rb = p.res + m0 * p.res_ld + (long long)n0 * sizeof(T);
+    const int pc = wn0 + (BF16 ? (fh & 1) * 16 + (fh >> 1) * 8 : fh * 4);           // first column of this lane's piece of pair 0
+    const uint32_t ro = (uint32_t)(wm0 + fr) * (uint32_t)p.res_ld + (uint32_t)pc * (uint32_t)sizeof(T);
+    const uint32_t oo = (uint32_t)(wm0 + fr) * (uint32_t)p.out_ld + (uint32_t)pc * (uint32_t)sizeof(T);
+    const int mleft = (int)min((long long)BM, p.M - m0) - wm0 - fr, nleft = min(BN, p.N - n0) - pc;    // rows / columns from this lane's first on
+    auto finish = [&](auto inner) {
+        auto whole = [&](int j, int i) { return inner.value || (j * 16 < mleft && i * 16 + P <= nleft); };
         // residual pieces come in two halves of the rows, the second requested before the first half's results are stored:
         // a load behind a store would wait for it
         constexpr int C = TM % 2 == 0 ? 2 : 1, CM = TM / C;
@@ -237,8 +239,12 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
 #pragma unroll
                 for (int i = 0; i < TN; i += 2) {
                     const char* q = rb + (long long)(c * CM + j) * 16 * p.res_ld + i * 16 * (int)sizeof(T) + ro;
-                    rv[j][i / 2] = *(const u32x4*)q;
-                    if constexpr (!BF16) rw[j][i / 2] = *(const u32x4*)(q + 64);
+                    rv[j][i / 2] = u32x4{0, 0, 0, 0};
+                    if (whole(c * CM + j, i)) __builtin_memcpy(&rv[j][i / 2], q, 16);
+                    if constexpr (!BF16) {
+                        rw[j][i / 2] = u32x4{0, 0, 0, 0};
+                        if (whole(c * CM + j, i + 1)) __builtin_memcpy(&rw[j][i / 2], q + 64, 16);
+                    }
                 }
         };
         fetch_res(0);
@@ -286,25 +292,33 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
 #pragma unroll
                 for (int i = 0; i < TN; i += 2) {
                     char* o = ob + (long long)(c * CM + j) * 16 * p.out_ld + i * 16 * (int)sizeof(T) + oo;
-                    *(u32x4*)o = ov[j][i / 2];
-                    if constexpr (!BF16) *(u32x4*)(o + 64) = ow[j][i / 2];
+                    if (whole(c * CM + j, i)) __builtin_memcpy(o, &ov[j][i / 2], 16);
+                    if constexpr (!BF16) {
+                        if (whole(c * CM + j, i + 1)) __builtin_memcpy(o + 64, &ow[j][i / 2], 16);
+                    }
                 }
         }
-    } else {
-        with_act(p.act, [&](auto mode) {                // an edge, or rows off 16-byte boundaries: element by element
+    };
+    if (m0 + BM <= p.M && n0 + BN <= p.N) finish(std::true_type{});
+    else finish(std::false_type{});
+    // the last N % P columns, element by element: one 16-wide tile of one wave column
+    const int tail = p.N / P * P;
+    if (tail < p.N && tail >= n0 + wn0 && tail < n0 + wn0 + TN * 16) {
+        with_act(p.act, [&](auto mode) {
             constexpr int ACT = decltype(mode)::value;
 #pragma unroll
-            for (int j = 0; j < TM; ++j) {
-                const long long m = m0 + wm0 + j * 16 + fr;
-                if (m >= p.M) continue;
-                T* o = (T*)(p.out + m * p.out_ld);
-                const T* q = (const T*)(p.res + m * p.res_ld);
+            for (int i = 0; i < TN; ++i) {
+                const int n = n0 + wn0 + i * 16 + fh * 4;
+                if ((tail - n0 - wn0) / 16 != i || n + 3 < tail) continue;
 #pragma unroll
-                for (int i = 0; i < TN; ++i) {
-                    const int n = n0 + wn0 + i * 16 + fh * 4;
+                for (int j = 0; j < TM; ++j) {
+                    const long long m = m0 + wm0 + j * 16 + fr;
+                    if (m >= p.M) continue;
+                    T* o = (T*)(p.out + m * p.out_ld);
+                    const T* q = (const T*)(p.res + m * p.res_ld);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        if (n + r >= p.N) continue;
+                        if (n + r < tail || n + r >= p.N) continue;
                         float v = activate<BF16, ACT>(acc[i][j][r]);
                         if (p.res) v += load_f32(q + n + r);
                         o[n + r] = (T)v;
@@ -432,7 +446,8 @@ static int launch_direct(LinK k, hipStream_t stream) {
 // Measured (bf16, us for 256 / 128 / 64): 23104 x 4096 x 1024 220 / 246 / 316, 10816 x 512 x 1024 31.7 / 22.3 / 26.9,
 // 2704 x 1024 x 512 42 / 12.4 / 9.6; f32 has no 256 x 256 (288 against 216 at 23104 x 1024 x 512: its registers do not fit).
 // Few outputs go to the direct kernel, which splits K inside a workgroup: up to 512 tiles of 16 x 16 (40 x 1024 x 1024: 4.1 against 6.7 in
-// 32 x 32 and 8.2 in 64 x 64), up to 256 of 32 x 32 (300 x 512 x 1024: 7.4 against 11.2; 700 x 512 x 512, 352 tiles: 9.0 against 7.9).
+// 32 x 32 and 8.2 in 64 x 64), up to 256 of 32 x 32 (300 x 512 x 1024: 7.4 against 11.2; 700 x 512 x 512, 352 tiles: 9.0 against 7.9), 512 in f32, whose products
+// take four times as long (300 x 512 x 1024: 10.8 against 24.6).
 // The direct kernel forms 64-bit addresses; the tile kernel offsets rows of a tile in 32 bits and takes strides up to 4 MB.
 template <bool BF16>
 static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
@@ -440,7 +455,7 @@ static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
     const long long kMaxStride = 1ll << 22;
     const bool wide = k.x_ld > kMaxStride || k.w_ld > kMaxStride || k.out_ld > kMaxStride || (k.res && k.res_ld > kMaxStride);
     if (tiles(16) <= 512) return aligned ? launch_direct<BF16, 1, 1, true>(k, stream) : launch_direct<BF16, 1, 1, false>(k, stream);
-    if (tiles(32) <= 256 || wide) return aligned ? launch_direct<BF16, 2, 2, true>(k, stream) : launch_direct<BF16, 2, 2, false>(k, stream);
+    if (tiles(32) <= (BF16 ? 256 : 512) || wide) return aligned ? launch_direct<BF16, 2, 2, true>(k, stream) : launch_direct<BF16, 2, 2, false>(k, stream);
     const double c256 = (double)((tiles(256) + 255) / 256) * 4.0, c128 = (double)((tiles(128) + 511) / 512) * 2.4, c64 = (double)((tiles(64) + 1023) / 1024) * 1.7;
     if constexpr (BF16) {
         if (aligned && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
@@ -473,7 +488,6 @@ extern "C" int yolo_linear(int dtype, const void* x, int64_t x_ld, const void* w
     k.x_ld = x_ld * z; k.w_ld = weight_ld * z; k.res_ld = residual_ld * z; k.out_ld = out_ld * z;
     k.M = M; k.N = N; k.K = K;
     k.bias_bf16 = bias_dtype == YOLO_DTYPE_BF16; k.act = activation;
-    k.vec_out = aligned16(out) && k.out_ld % 16 == 0 && (!residual || (aligned16(residual) && k.res_ld % 16 == 0));
     k.ntm = k.ntn = 0;
     const bool al = aligned16(x) && aligned16(weight) && k.x_ld % 16 == 0 && k.w_ld % 16 == 0 && (long long)K * z % 16 == 0;
     return dtype == YOLO_DTYPE_BF16 ? launch_linear<true>(k, al, (hipStream_t)stream) : launch_linear<false>(k, al, (hipStream_t)stream);

@@ -30,7 +30,7 @@ struct RopeK {
     float eps;
 };
 
-constexpr int kRopeTable = 4096;    // (cos, sin) pairs a workgroup keeps in LDS: 32 KB
+constexpr int kRopeTable = 512;     // (cos, sin) pairs a workgroup computes, two a thread, and keeps in LDS; a token has at most 128
 
 // cos / sin of every (token, pair) of this workgroup and the norm weights -> LDS
 __device__ __forceinline__ void rope_tables(const RopeK& p, const RopeSide& s, int t0, int nt, float2* cs, float* wt) {
