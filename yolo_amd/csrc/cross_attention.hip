@@ -416,18 +416,17 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
     }
 }
 
-// Joins the key splits of a row: WPR waves per row, lane = split for the maxima and sums, lane + 64 i = element for the results; a
-// wave adds every WPR-th split with four loads in flight, the waves' sums are added in order: the result does not depend on the launch.
-constexpr int kMaxSplits = 64;
+// Joins the key splits of a row: a workgroup of WPR waves per row, lane = split for the maxima and sums, lane + 64 i = element for the
+// results; a wave adds every WPR-th split with four loads in flight, the waves' sums are added in order: the result does not depend on
+// the launch.
+constexpr int kMaxSplits = 64, WPR = 4;
 
-template <bool BF16, int WPR>
+template <bool BF16>
 __global__ __launch_bounds__(256) void cross_attention_join_kernel(AttnK p) {
     typedef typename Elem<BF16>::type T;
-    __shared__ float sums[WPR > 1 ? WPR : 1][256];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w0 = wave % WPR;
-    const long long total = (long long)p.B * p.Lq * p.Hq;
-    const long long row = (long long)blockIdx.x * (4 / WPR) + wave / WPR;
-    if (row >= total) return;                               // WPR = 4: the whole workgroup
+    __shared__ float sums[WPR][256];
+    const int lane = threadIdx.x & 63, w0 = threadIdx.x >> 6;
+    const long long total = (long long)p.B * p.Lq * p.Hq, row = blockIdx.x;
     const bool have = lane < p.splits;
     const float2 ml = have ? p.ml[lane * total + row] : make_float2(-__builtin_inff(), -1.0f);
     const bool kept = have && ml.y != -1.0f;                // a NaN sum is kept
@@ -457,21 +456,59 @@ __global__ __launch_bounds__(256) void cross_attention_join_kernel(AttnK p) {
             for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(ws, v[u][i], o[i]);
         }
     }
-    if constexpr (WPR > 1) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sums[w0][lane + 64 * i] = o[i];
-        __syncthreads();
-        if (w0) return;
+    for (int i = 0; i < 4; ++i) sums[w0][lane + 64 * i] = o[i];
+    __syncthreads();
+    if (w0) return;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int x = 1; x < WPR; ++x) o[i] += sums[x][lane + 64 * i];
-    }
+        for (int x = 1; x < WPR; ++x) o[i] += sums[x][lane + 64 * i];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int d = lane + 64 * i;
         if (d < p.D) ((T*)p.out)[row * p.D + d] = (T)(any ? o[i] / l : 0.f);
     }
+}
+
+// The same for up to 8 splits and many rows: a thread per four elements, all its loads in flight.
+template <bool BF16>
+__global__ __launch_bounds__(256) void cross_attention_join_rows_kernel(AttnK p) {
+    typedef typename Elem<BF16>::type T;
+    const long long total = (long long)p.B * p.Lq * p.Hq;
+    const int quads = p.D / 4;
+    const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id / quads;
+    const int d = (int)(id - row * quads) * 4;
+    if (row >= total) return;
+    float2 ml[8];
+    f32x4 v[8];
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        ml[s] = s < p.splits ? p.ml[s * total + row] : make_float2(-__builtin_inff(), -1.0f);
+        v[s] = s < p.splits ? *(const f32x4*)(p.part + (s * total + row) * p.D + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    float m = -__builtin_inff(), l = 0.f;
+    bool any = false;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+        if (ml[s].y != -1.0f) {
+            m = fmaxf(m, ml[s].x);
+            any = true;
+        }
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+        if (ml[s].y == -1.0f) continue;
+        const float w = ml[s].x != -__builtin_inff() ? __builtin_amdgcn_exp2f((ml[s].x - m) * p.scale2) : ml[s].y == 0.f ? 0.f : 1.f;
+        l += w * ml[s].y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = __builtin_fmaf(w, v[s][j], o[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = any ? o[j] / l : 0.f;
+    T* out = (T*)p.out + row * p.D + d;
+    if constexpr (BF16) *(u32x2*)out = u32x2{pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3])};
+    else *(f32x4*)out = o;
 }
 
 // ---- plan: the tile shape and the number of key splits, by sizes and type alone ---------------------------------------------------
@@ -499,11 +536,18 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) a.waves = 8;
     a.rtiles = (int)rtiles(a.waves);
     const long long blocks = a.rtiles * groups;
-    // workgroups at a time: by registers and LDS two of four waves to a CU in bf16, one where a wave has the whole register file
-    // or, in f32, the matrix cores are busy with one
-    const long long slots = a.waves == 1 ? 1024 : a.waves == 4 && bf16 && a.dc < 256 ? 512 : 256;
-    // a one-wave workgroup alone on its SIMD: 1.07 us a tile (64 of 64, bf16), its loads' latency
-    const double tile_us = (bf16 ? 0.4 + 0.6 * a.dc / 128 * a.kt / 64 : 3.5 * a.dc / 64 * a.kt / 64) * (a.waves == 1 ? 1.5 : 1.0);
+    // a round: 256 workgroups, one to a CU, take `one` us a tile (latency), 512 of four waves `two` (one where a wave has the whole
+    // register file); one-wave workgroups run as many to a CU as their LDS allows
+    const int row_bytes = a.dc <= 32 ? (bf16 ? 64 : 128) : a.dc <= 64 ? (bf16 ? 128 : 256) : a.dc <= 128 ? (bf16 ? 256 : 512) : (bf16 ? 512 : 1024);
+    const double part = a.dc / 64.0 * a.kt / 64.0;
+    const bool pairs = a.waves == 4 && a.dc < 256 && (bf16 || a.dc <= 64);
+    const double one = a.waves == 1 ? (bf16 ? 0.3 + 0.8 * part : 5.0 * part) : a.waves == 8 ? 0.6 + 0.75 * part : bf16 ? 0.5 + 0.45 * part : 4.8 * part;
+    const double two = bf16 ? 0.6 + 0.8 * part : 7.5 * part;
+    const long long per_cu = a.waves != 1 ? 1 : 160 * 1024 / (4 * a.kt * row_bytes) < 4 ? 160 * 1024 / (4 * a.kt * row_bytes) : 4;
+    auto tile_us = [&](long long n) {                                               // n workgroups, one tile each
+        if (!pairs) return rounds(n, 256 * per_cu) * one;
+        return n / 512 * two + (n % 512 == 0 ? 0.0 : n % 512 <= 256 ? one : two);
+    };
     const double join_fixed_us = a.waves == 1 ? 7.0 : 4.0;                          // where latency counts also the launch on the host
     const double join_us = 4e-6 * 2 * B * Lq * (double)Hq * D / 4;                  // of one more split, at 4 TB/s
     double best = 0;
@@ -511,7 +555,7 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     a.tps = tiles;
     for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
         const int tps = (tiles + s - 1) / s, splits = (tiles + tps - 1) / tps;
-        const double t = (double)rounds(blocks * splits, slots) * (tps + 1) * tile_us + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
+        const double t = tile_us(blocks * splits) * (tps + 1.5) + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
         if (s == 1 || t < best) {
             best = t;
             a.splits = splits;
@@ -566,11 +610,10 @@ static int launch_attn(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
         default: rc = launch_attn_dc<BF16, 256>(p, a, stream); break;
     }
     if (rc != YOLO_OK || p.splits == 1) return rc;
-    // four waves per row where a row has more than one batch of loads
-    const unsigned long long rows = (unsigned long long)p.B * p.Lq * p.Hq, blocks = p.splits > 4 ? rows : (rows + 3) / 4;
+    const unsigned long long rows = (unsigned long long)p.B * p.Lq * p.Hq, blocks = p.splits > 8 ? rows : (rows * (p.D / 4) + 255) / 256;
     YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 rows");
-    if (p.splits > 4) hipLaunchKernelGGL((cross_attention_join_kernel<BF16, 4>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((cross_attention_join_kernel<BF16, 1>), dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    if (p.splits > 8) hipLaunchKernelGGL(cross_attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL(cross_attention_join_rows_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
