@@ -546,3 +546,53 @@ def test_attention_long_states(L, t, b, lq, lk, hq, hk, d):
     assert got[:, :, :hq // hk].isnan().all()
     if hk > 1:
         assert torch.isfinite(got[:, :, hq // hk:]).all()
+
+
+def test_split_attention_in_graphs_on_two_streams(L):
+    """Key splits use a workspace: two captured graphs and eager calls on other streams at the same time keep to their own."""
+    cases = [qkv(BF16, 2, 1, 6000, 8, 2, 64, 200), qkv(F32, 1, 90, 4000, 4, 4, 64, 210)]
+    from yolo_amd import _lib
+    for code, (q, k, v) in zip((1, 0), cases):
+        assert _lib.lib().yolo_cross_attention_workspace_bytes(code, q.shape[0], q.shape[1], k.shape[1], q.shape[2], k.shape[2], 64) > 0
+    want = [L.cross_attention(*c) for c in cases]
+    graphs = []
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = L.cross_attention(*c)
+        graphs.append((g, out))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, out in graphs:
+            out.zero_()
+        torch.cuda.synchronize()
+        for s, (g, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            eager = [L.cross_attention(*c) for c in cases]
+        here = [L.cross_attention(*c) for c in cases]
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(graphs[i][1], want[i]) and torch.equal(eager[i], want[i]) and torch.equal(here[i], want[i])
+
+
+def test_attention_workspace_is_checked(L):
+    """The C entry: too small a workspace is an error before any launch; an unaligned call needs none."""
+    import ctypes
+    from yolo_amd import _lib, _tensor
+    lib = _lib.lib()
+    q, k, v = qkv(BF16, 1, 1, 6000, 2, 2, 64, 220)
+    need = lib.yolo_cross_attention_workspace_bytes(1, 1, 1, 6000, 2, 2, 64)
+    st = (ctypes.c_int64 * 3)(k.stride(0), k.stride(1), k.stride(2))
+    qs = (ctypes.c_int64 * 3)(q.stride(0), q.stride(1), q.stride(2))
+    out, ws = torch.zeros_like(q), _tensor.workspace(need)
+
+    def call(w, n):
+        return lib.yolo_cross_attention(1, q.data_ptr(), qs, k.data_ptr(), st, v.data_ptr(), st, None, None, 1, 1, 6000, 2, 2, 64, 0.125,
+                                        out.data_ptr(), w, n, _tensor.stream_ptr())
+    assert call(None, 0) == -5 and call(ws.data_ptr(), need - 1) == -5 and call(ws.data_ptr() + 8, need) == -5
+    assert b"workspace" in lib.yolo_last_error() and (out == 0).all()
+    assert call(ws.data_ptr(), need) == 0
+    assert torch.equal(out, L.cross_attention(q, k, v))

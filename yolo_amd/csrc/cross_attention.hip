@@ -108,7 +108,7 @@ __global__ __launch_bounds__(256) void cross_attention_general_kernel(AttnK p) {
 }
 
 // ---- tiles on the matrix cores --------------------------------------------------------------------------------------------------
-// A workgroup of WAVES waves takes 32 NQ WAVES query rows of one (image, key head) - row r is query r / G, head r % G of the group,
+// A workgroup of WAVES waves takes 32 WAVES query rows of one (image, key head) - row r is query r / G, head r % G of the group,
 // so that the heads that share k and v share their tiles - and walks KT keys at a time; k and v tiles are double-buffered in
 // LDS by DMA, one barrier per tile.
 //
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(256) void cross_attention_general_kernel(AttnK p) {
 //
 // The running maximum is only raised when a score exceeds it by 2^8 in weight: weights stay below 2^8, which costs no precision
 // (they are floating point) and most tiles skip the rescaling of o.
-// bf16: the weights are rounded to bf16 for the second product, at most 2^-9 of each, independent in sign, which is of the size of the
+// bf16: the weights are rounded to bf16 for the second product, at most 2^-8 of each and of either sign, which is the size of the
 // rounding of the result; their sum is taken of the f32 values.
 //
 // LDS rows are the next power of two of the head size.  k: 16-byte piece c of a row at c ^ f(row) so that 16 rows' pieces fall on
@@ -144,7 +144,7 @@ template <bool BF16, int DC> struct AttnTile {
     }
 };
 
-template <bool BF16, int DC, int WAVES, int NQ, int MW>
+template <bool BF16, int DC, int WAVES, int MW>
 __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(AttnK p) {
     typedef typename Elem<BF16>::type T;
     typedef AttnTile<BF16, DC> L;
@@ -170,15 +170,12 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
     const int t1 = min((n + KT - 1) / KT, t0 + p.tps);
 
     // query rows of this wave -> registers (operand layout: column = row of q, 16-byte piece 2 step + half)
-    int row[NQ];
-    long long orow[NQ];                                     // row of the packed output
-    u32x4 fq[NQ][QS];
-#pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-        row[x] = rt * (32 * NQ * WAVES) + (wave * NQ + x) * 32 + col;
-        const int r = min(row[x], rows - 1);
-        const int l = r / p.G, h = hk * p.G + r % p.G;
-        orow[x] = ((long long)b * p.Lq + l) * p.Hq + h;
+    const int row = rt * (32 * WAVES) + wave * 32 + col;
+    long long orow;                                         // row of the packed output
+    u32x4 fq[QS];
+    {
+        const int r = min(row, rows - 1), l = r / p.G, h = hk * p.G + r % p.G;
+        orow = ((long long)b * p.Lq + l) * p.Hq + h;
         const char* q = p.q + (b * p.qb + l * p.ql + h * p.qh) * (long long)sizeof(T);
 #pragma unroll
         for (int s = 0; s < QS; ++s) {
@@ -186,21 +183,16 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
             u32x4 v = *(c * P < p.D ? (const u32x4*)(q + c * 16) : &kZeroPiece);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = (v[j] & p.q_and) ^ p.q_xor;
-            fq[x][s] = v;
+            fq[s] = v;
         }
     }
 
-    f32x16 o[NQ][DT];
-    float mref[NQ], sum[NQ];
+    f32x16 o[DT];
+    float mref = -__builtin_inff(), sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-        mref[x] = -__builtin_inff();
-        sum[x] = 0.f;
+    for (int i = 0; i < DT; ++i)
 #pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[x][i][r] = 0.f;
-    }
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
 
     // staging: thread covers slot tid % PCS of rows tid / PCS + RPI i
     const int r0 = tid / PCS, slot = tid % PCS;
@@ -264,26 +256,21 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
         const char* kt = lds + buf * L::TILE;
         const char* vt = lds + (2 + buf) * L::TILE;
 
-        f32x16 s[NQ][KB];
+        f32x16 s[KB];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-            for (int x = 0; x < NQ; ++x)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[x][kb][r] = 0.f;
+            for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
             const int key = kb * 32 + col;
 #pragma unroll
             for (int st = 0; st < QS; ++st) {
                 const u32x4 fk = *(const u32x4*)(kt + key * L::ROW + L::kpiece(key, 2 * st + half) * 16);
+                if constexpr (BF16) {
+                    s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fk), __builtin_bit_cast(bf16x8, fq[st]), s[kb], 0, 0, 0);
+                } else {
+                    const f32x4 a = __builtin_bit_cast(f32x4, fk), q = __builtin_bit_cast(f32x4, fq[st]);
 #pragma unroll
-                for (int x = 0; x < NQ; ++x) {
-                    if constexpr (BF16) {
-                        s[x][kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, fk), __builtin_bit_cast(bf16x8, fq[x][st]), s[x][kb], 0, 0, 0);
-                    } else {
-                        const f32x4 a = __builtin_bit_cast(f32x4, fk), q = __builtin_bit_cast(f32x4, fq[x][st]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) s[x][kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], q[j], s[x][kb], 0, 0, 0);
-                    }
+                    for (int j = 0; j < 4; ++j) s[kb] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], q[j], s[kb], 0, 0, 0);
                 }
             }
         }
@@ -293,58 +280,51 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const bool in = (kept >> (kb * 32 + 8 * (r >> 2) + 4 * half + (r & 3))) & 1;
-#pragma unroll
-                    for (int x = 0; x < NQ; ++x) s[x][kb][r] = in ? s[x][kb][r] : -__builtin_inff();
+                    s[kb][r] = in ? s[kb][r] : -__builtin_inff();
                 }
         }
         any |= kept != 0;
         kept = next;
 
+        float mt = s[0][0];
 #pragma unroll
-        for (int x = 0; x < NQ; ++x) {
-            float mt = s[x][0][0];
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const bool raise = (mt - mref) * p.scale2 > 8.f;    // false while both are -inf
+        if (__any(raise)) {
+            const float mn = fmaxf(mref, mt);
+            const float c = mref == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mref - mn) * p.scale2);
+            mref = mn;
+            sum *= c;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[x][kb][r]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32));
-            const bool raise = (mt - mref[x]) * p.scale2 > 8.f;                     // false while both are -inf
-            if (__any(raise)) {
-                const float mn = fmaxf(mref[x], mt);
-                const float c = mref[x] == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f((mref[x] - mn) * p.scale2);
-                mref[x] = mn;
-                sum[x] *= c;
+            for (int i = 0; i < DT; ++i)
 #pragma unroll
-                for (int i = 0; i < DT; ++i)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[x][i][r] *= c;
-            }
-            const float base = mref[x] == -__builtin_inff() ? 0.f : mref[x] * p.scale2;
-            float st = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][kb][r], p.scale2, -base));
-                    s[x][kb][r] = e;
-                    st += e;
-                }
-            sum[x] += st;
+                for (int r = 0; r < 16; ++r) o[i][r] *= c;
         }
+        const float base = mref == -__builtin_inff() ? 0.f : mref * p.scale2;
+        float st = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], p.scale2, -base));
+                s[kb][r] = e;
+                st += e;
+            }
+        sum += st;
 
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             if constexpr (BF16) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {               // 16 keys: registers 8 g .. 8 g + 7
-                    bf16x8 fp[NQ];
+                    bf16x8 fp;
+                    u32x4 pk;
 #pragma unroll
-                    for (int x = 0; x < NQ; ++x) {
-                        u32x4 pk;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(s[x][kb][8 * g + 2 * j], s[x][kb][8 * g + 2 * j + 1]);
-                        fp[x] = __builtin_bit_cast(bf16x8, pk);
-                    }
+                    for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(s[kb][8 * g + 2 * j], s[kb][8 * g + 2 * j + 1]);
+                    fp = __builtin_bit_cast(bf16x8, pk);
                     // lane's address for the transposed read: key row (lane / 4) % 4 of its four keys, 4 elements at 4 (lane % 4)
                     const int key = kb * 32 + 16 * g + 4 * half + ((lane >> 2) & 3);
 #pragma unroll
@@ -357,8 +337,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
                             (__attribute__((address_space(3))) char*)vt + (key + 8) * L::ROW + L::vpiece(key + 8, c) * 16 + w));
                         typedef short s16x8 __attribute__((ext_vector_type(8)));
                         const bf16x8 fv = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                        for (int x = 0; x < NQ; ++x) o[x][i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv, fp[x], o[x][i], 0, 0, 0);
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv, fp, o[i], 0, 0, 0);
                     }
                 }
             } else {
@@ -369,8 +348,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
                     for (int i = 0; i < DT; ++i) {
                         const int e = i * 32 + col;
                         const float fv = *(const float*)(vt + key * L::ROW + L::vpiece(key, e / 4) * 16 + (e & 3) * 4);
-#pragma unroll
-                        for (int x = 0; x < NQ; ++x) o[x][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(fv, s[x][kb][r], o[x][i], 0, 0, 0);
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(fv, s[kb][r], o[i], 0, 0, 0);
                     }
                 }
             }
@@ -378,39 +356,36 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
     }
 
     const long long total = (long long)p.B * p.Lq * p.Hq;
+    const float l = sum + __shfl_xor(sum, 32);
+    const bool in = row < rows;
+    const bool parts = p.part != nullptr;
+    const float f = parts ? 1.0f : any ? 1.0f / l : 0.f;
+    if (in && parts && half == 0) p.ml[split * total + orow] = make_float2(mref, any ? l : -1.0f);
 #pragma unroll
-    for (int x = 0; x < NQ; ++x) {
-        const float l = sum[x] + __shfl_xor(sum[x], 32);
-        const bool in = row[x] < rows;
-        const bool parts = p.part != nullptr;
-        const float f = parts ? 1.0f : any ? 1.0f / l : 0.f;
-        if (in && parts && half == 0) p.ml[split * total + orow[x]] = make_float2(mref[x], any ? l : -1.0f);
+    for (int i = 0; i < DT; ++i) {
 #pragma unroll
-        for (int i = 0; i < DT; ++i) {
+        for (int g = 0; g < 2; ++g) {
+            // registers 8 g + 0..3 and 8 g + 4..7 are elements 16 g + 4 half + 0..3 and + 8: after the exchange of lane halves a lane
+            // holds 8 consecutive elements, 16 g + 8 half ..
+            float v[8];
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                // registers 8 g + 0..3 and 8 g + 4..7 are elements 16 g + 4 half + 0..3 and + 8: after the exchange of lane halves a lane
-                // holds 8 consecutive elements, 16 g + 8 half ..
-                float v[8];
+            for (int j = 0; j < 4; ++j) {
+                const float a = o[i][8 * g + j] * f, c = o[i][8 * g + 4 + j] * f;
+                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(c), false, false);
+                v[j] = __uint_as_float(sw[0]);
+                v[4 + j] = __uint_as_float(sw[1]);
+            }
+            const int d = i * 32 + 16 * g + 8 * half;
+            if (!in || d >= p.D) continue;              // D is whole groups of 8
+            if (parts || !BF16) {
+                float* dst = parts ? p.part + (split * total + orow) * p.D + d : (float*)p.out + orow * p.D + d;
+                *(f32x4*)dst = f32x4{v[0], v[1], v[2], v[3]};
+                *(f32x4*)(dst + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            } else {
+                u32x4 pk;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float a = o[x][i][8 * g + j] * f, c = o[x][i][8 * g + 4 + j] * f;
-                    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(c), false, false);
-                    v[j] = __uint_as_float(sw[0]);
-                    v[4 + j] = __uint_as_float(sw[1]);
-                }
-                const int d = i * 32 + 16 * g + 8 * half;
-                if (!in || d >= p.D) continue;              // D is whole groups of 8
-                if (parts || !BF16) {
-                    float* dst = parts ? p.part + (split * total + orow[x]) * p.D + d : (float*)p.out + orow[x] * p.D + d;
-                    *(f32x4*)dst = f32x4{v[0], v[1], v[2], v[3]};
-                    *(f32x4*)(dst + 4) = f32x4{v[4], v[5], v[6], v[7]};
-                } else {
-                    u32x4 pk;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
-                    *(u32x4*)((__bf16*)p.out + orow[x] * p.D + d) = pk;
-                }
+                for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(v[2 * j], v[2 * j + 1]);
+                *(u32x4*)((__bf16*)p.out + orow * p.D + d) = pk;
             }
         }
     }
@@ -513,15 +488,16 @@ __global__ __launch_bounds__(256) void cross_attention_join_rows_kernel(AttnK p)
 
 // ---- plan: the tile shape and the number of key splits, by sizes and type alone ---------------------------------------------------
 struct AttnPlan {
-    int dc, waves, nq, kt, rtiles, splits, tps;
+    int dc, waves, kt, rtiles, splits, tps;
     size_t bytes;
 };
 
 // The number of key splits S is the one of least modelled time, in microseconds: rounds of workgroups times the tiles of one, and for
 // S > 1 the join's launch and the traffic of the partial results.  Measured (bf16, us at S = 1 / 2 / 4): 32 x 100 queries of 8 heads of 64 over
-// 3549 keys 74 / 65 / 68, 16 x 100 of 128 over 3549 101 / 69 / 64, 64 x 2704 of 64 over 80 keys 133 / 710 / 710; one query of 16
-// heads of 64, 4 key heads: 9.1 at S = 1, 8.5 at 5 over 300 keys; 28 at 1, 8.9 at 12 over 1444; 64 at 1, 10 at 28 over 3549.  Eight waves share a tile's loads where their larger row tiles still fill the CUs as
-// well (8 x 2704 queries of 8 heads of 128: 524 against 553), not over few tiles (80 keys, above: 153).
+// 3549 keys 76 / 60 / 68, 16 x 100 of 128 over 3549 100 / 67 / 63, 64 x 2704 of 64 over 80 keys 126 / 437 / 437; one query of 16
+// heads of 64, 4 key heads: 9.1 at S = 1, 8.5 at 5 over 300 keys; 28 at 1, 8.9 at 12 over 1444; 64 at 1, 10 at 28 over 3549.
+// Eight waves share a tile's loads where their larger row tiles still fill the CUs as well (8 x 2704 queries of 8 heads of 128: 524
+// against 553), not over few tiles (80 keys, above: 153).
 static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
     AttnPlan a;
     const bool bf16 = dtype == YOLO_DTYPE_BF16;
@@ -531,7 +507,6 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     auto rtiles = [&](int waves) { return (rows + 32 * waves - 1) / (32 * waves); };
     auto rounds = [](long long blocks, long long slots) { return (blocks + slots - 1) / slots; };
     a.waves = rows <= 32 && a.dc < 256 ? 1 : 4;
-    a.nq = 1;
     const int tiles = (Lk + a.kt - 1) / a.kt;
     if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) a.waves = 8;
     a.rtiles = (int)rtiles(a.waves);
@@ -568,7 +543,7 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
 
 // MW: waves per SIMD the register budget is cut for.  Two hide each other's latencies where the tiles fill the GPU (D = 128, four waves:
 // 804 us at one, 553 at two); one-wave workgroups run one to a SIMD, and 256 elements of o, q and their tiles need all 512 registers
-template <bool BF16, int DC, int WAVES, int NQ, int MW = (WAVES == 1 || DC == 256 || (!BF16 && DC > 64)) ? 1 : 2>
+template <bool BF16, int DC, int WAVES, int MW = (WAVES == 1 || DC == 256 || (!BF16 && DC > 64)) ? 1 : 2>
 static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
     constexpr int kLds = AttnTile<BF16, DC>::LDS;
     if (kLds > 64 * 1024) {
@@ -576,14 +551,14 @@ static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
         int dev = 0;
         YOLO_HIP_CHECK(hipGetDevice(&dev));
         if (dev >= 16 || !attr_done[dev]) {
-            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, NQ, MW>,
+            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, MW>,
                                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
             if (dev < 16) attr_done[dev] = true;
         }
     }
     const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk;
     YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 workgroups");
-    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, NQ, MW>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
+    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, MW>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
@@ -591,12 +566,12 @@ static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
 template <bool BF16, int DC>
 static int launch_attn_dc(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
     if constexpr (BF16 && (DC == 64 || DC == 96 || DC == 128)) {
-        if (a.waves == 8) return launch_attn_tile<BF16, DC, 8, 1>(p, stream);
+        if (a.waves == 8) return launch_attn_tile<BF16, DC, 8>(p, stream);
     }
     if constexpr (DC < 256) {
-        if (a.waves == 1) return launch_attn_tile<BF16, DC, 1, 1>(p, stream);
+        if (a.waves == 1) return launch_attn_tile<BF16, DC, 1>(p, stream);
     }
-    return launch_attn_tile<BF16, DC, 4, 1>(p, stream);
+    return launch_attn_tile<BF16, DC, 4>(p, stream);
 }
 
 template <bool BF16>
@@ -623,7 +598,8 @@ static int launch_attn(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
 extern "C" size_t yolo_cross_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
     using namespace yolo;
     if ((dtype != YOLO_DTYPE_F32 && dtype != YOLO_DTYPE_BF16) || B <= 0 || Lq <= 0 || Lk <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk ||
-        D <= 0 || D > 256 || D % 8 || (unsigned long long)B * Lq >= (1ull << 31) || Hq > 65536 || (long long)Lq * (Hq / Hk) >= (1ll << 31))
+        D <= 0 || D > 256 || D % 8 || (unsigned long long)B * Lq >= (1ull << 31) || Hq > 65536 || Lk > (1 << 30) ||
+        (long long)Lq * (Hq / Hk) > (1ll << 30))
         return 0;
     return attn_plan(dtype, B, Lq, Lk, Hq, Hk, D).bytes;
 }
@@ -643,7 +619,8 @@ extern "C" int yolo_cross_attention(int dtype, const void* q, const int64_t* q_s
     YOLO_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out) & (z - 1)) == 0 && ((uintptr_t)key_lens & 3) == 0,
                  YOLO_ERR_ARG, "cross_attention: a pointer is not aligned to its element");
     YOLO_REQUIRE((unsigned long long)B * Lq < (1ull << 31) && Hq <= 65536, YOLO_ERR_UNSUPPORTED, "cross_attention: B * Lq must be below 2^31, at most 65536 heads");
-    YOLO_REQUIRE(std::isfinite(scale), YOLO_ERR_ARG, "cross_attention: scale must be finite");
+    YOLO_REQUIRE(std::isfinite(scale * 1.44269504f), YOLO_ERR_ARG, "cross_attention: scale must be finite");
+    YOLO_REQUIRE(Lk <= (1 << 30), YOLO_ERR_UNSUPPORTED, "cross_attention: at most 2^30 keys");
     AttnK p;
     p.q = (const char*)q; p.k = (const char*)k; p.v = (const char*)v; p.out = (char*)out;
     p.lens = key_lens; p.mask = key_mask;
@@ -656,7 +633,7 @@ extern "C" int yolo_cross_attention(int dtype, const void* q, const int64_t* q_s
     p.B = B; p.Lq = Lq; p.Lk = Lk; p.Hq = Hq; p.Hk = Hk; p.D = D; p.G = Hq / Hk; p.scale = scale;
     p.part = nullptr; p.ml = nullptr; p.q_and = ~0u; p.q_xor = 0; p.scale2 = 0.f; p.rtiles = 0; p.splits = 1; p.tps = 0;
     // the matrix-core kernels read whole 16-byte pieces of rows and hold the rows of a head group in 32 bits
-    bool fast = Lk > 0 && D % 8 == 0 && aligned16(out) && (long long)Lq * p.G < (1ll << 31);
+    bool fast = Lk > 0 && D % 8 == 0 && aligned16(out) && (long long)Lq * p.G <= (1ll << 30);
     const void* base[3] = {q, k, v};
     const int64_t* st[3] = {q_strides, k_strides, v_strides};
     for (int i = 0; fast && i < 3; ++i)
