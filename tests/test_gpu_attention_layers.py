@@ -596,3 +596,33 @@ def test_attention_workspace_is_checked(L):
     assert b"workspace" in lib.yolo_last_error() and (out == 0).all()
     assert call(ws.data_ptr(), need) == 0
     assert torch.equal(out, L.cross_attention(q, k, v))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("d,r", [(64, 16), (64, 32), (64, 48), (96, 64), (128, 32), (256, 128), (80, 16), (48, 40)])
+def test_qk_partial_rotation(L, t, d, r):
+    """rotary_dim below the head size, in whole pieces (register kernel) and not (general one)."""
+    q, k = rand((2, 21, 5, d), t, 230), rand((2, 33, 2, d), t, 231)
+    f, w = L.rope_frequencies(r, axes=2), rand((d,), t, 232)
+    for il in (False, True):
+        check_qk(L, q, k, w, w, f, grid_positions(21, 2, 2, 3), grid_positions(33, 2, 2), 2, il)
+
+
+def test_unaligned_attention_through_the_c_entry(L):
+    """Rows off 16-byte boundaries straight into the C entry (the Python function copies them): the general kernel, no workspace."""
+    import ctypes
+    from yolo_amd import _lib, _tensor
+    for t, code in ((F32, 0), (BF16, 1)):
+        big = rand((2, 70, 3, 67), t, 240)
+        q, k, v = big[:, :9, :, 1:65], big[:, 9:, :, 2:66], big[:, 9:, :, 3:67]
+        st = [(ctypes.c_int64 * 3)(*x.stride()[:3]) for x in (q, k, v)]
+        lens, mask = torch.tensor([61, 20], dtype=torch.int32, device="cuda"), torch.ones((2, 61), dtype=torch.bool, device="cuda")
+        mask[0, ::3] = False
+        out = torch.full((2, 9, 3, 64), 9.0, dtype=t, device="cuda")
+        _lib.check(_lib.lib().yolo_cross_attention(code, q.data_ptr(), st[0], k.data_ptr(), st[1], v.data_ptr(), st[2], lens.data_ptr(),
+                                                   mask.data_ptr(), 2, 9, 61, 3, 3, 64, 0.125, out.data_ptr(), None, 0, _tensor.stream_ptr()))
+        want = L.cross_attention(q, k, v, key_lens=lens, key_mask=mask)
+        # the two kernels differ by their roundings: one of the result and, in bf16, one of each weight
+        u = torch.finfo(t).eps / 2
+        a = L.cross_attention(q, k, v.abs(), key_lens=lens, key_mask=mask).double()
+        within(out, want.double(), 2 * u * want.double().abs() + (2.0 ** -16 + (2 * u if t == BF16 else 0)) * 2 * a, t)

@@ -106,9 +106,10 @@ __global__ __launch_bounds__(256) void qk_norm_rope_general_kernel(RopeK p) {
     }
 }
 
-// The usual layout: rotary_dim = D (or no rotation), D whole pairs of 16-byte pieces, aligned rows.  A lane holds two pieces whose
-// elements are each other's partners - pieces c and c + D/2 of a row, or neighbours if interleaved - so that the rotation needs no
-// exchange; LPR = D / (2 pieces) lanes, rounded up to a power of two, make a row, and its sum of squares is log2(LPR) lane exchanges.
+// The usual layout: D and rotary_dim whole pairs of 16-byte pieces, aligned rows.  A lane holds two pieces whose elements are each
+// other's partners - elements c P .. and R/2 + c P .. of a row, or neighbours if interleaved or past rotary_dim - so that the rotation
+// needs no exchange; LPR = D / (2 pieces) lanes, rounded up to a power of two, make a row, and its sum of squares is log2(LPR) lane
+// exchanges.
 // Bandwidth bounds it: a workgroup issues its first row loads before it computes the table (one sine / cosine per thread or so,
 // shared by all heads of a token).
 template <bool BF16>
@@ -150,7 +151,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeK p) {
     const int nt = min(s.tpb, s.tokens - t0), rows = nt * s.H;
     const int c = threadIdx.x % LPR, rw = threadIdx.x / LPR;
     const bool lane_in = c * 2 * P < p.D;                       // D / (2 P) lanes of the LPR hold pieces
-    const int da = IL ? 2 * c * P : c * P, db = IL ? da + P : da + p.D / 2;
+    const bool turned = c * 2 * P < p.R;                        // the lanes before the first that is not hold R elements
+    const int da = IL || !turned ? 2 * c * P : c * P, db = IL || !turned ? da + P : da + p.R / 2;
     u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
     int tl = 0, h = 0;
     auto load = [&](int r) {
@@ -192,8 +194,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(RopeK p) {
             u[j] *= rs * wa[j];
             v[j] *= rs * wb[j];
         }
-        if (p.freq) {
-            const float2* t = cs + tc * (p.D / 2) + c * P;      // pairs c P .. c P + P - 1 in either layout
+        if (turned) {
+            const float2* t = cs + tc * (p.R / 2) + c * P;      // pairs c P .. c P + P - 1 in either layout
 #pragma unroll
             for (int j = 0; j < P; ++j) {
                 const float2 w = t[j];
@@ -257,7 +259,7 @@ extern "C" int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const i
     const int piece = 16 / z;
     // lanes per row of the register kernel, 0: general kernel
     int lpr = 0;
-    if (D % (2 * piece) == 0 && (rotary_dim == 0 || rotary_dim == D))
+    if (D % (2 * piece) == 0 && rotary_dim % (2 * piece) == 0)
         for (lpr = 1; lpr * 2 * piece < D;) lpr *= 2;
     for (int i = 0; i < 2 && lpr; ++i) {
         const int64_t* st = i ? k_strides : q_strides;

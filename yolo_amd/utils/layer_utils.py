@@ -16,6 +16,7 @@ from __future__ import division, print_function
 
 import contextlib
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -272,6 +273,14 @@ def _heads(x, name):
     return x, _Strides(st[0], st[1], st[2])
 
 
+def _whole_rows(x):
+    """x [B, L, H, D] itself if all its rows start on 16 bytes, which the matrix-core kernels need, else a copy."""
+    st, z = x.stride(), x.element_size()
+    if (x.data_ptr() | st[0] * z | st[1] * z | st[2] * z) & 15:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
 def _positions(p, B, L, axes, name, dev):
     """-> (contiguous tensor, batched).  [L] / [B, L] for one axis, [L, 2] / [B, L, 2] for two; a trailing 1 is allowed for one."""
     p = _dev(p, name, dev)
@@ -342,23 +351,33 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, frequencies=None, q_positio
     return qo, ko
 
 
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(*sizes):
+    return _lib.lib().yolo_cross_attention_workspace_bytes(*sizes)
+
+
 def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     """softmax(scale * q k^T) v: q [B, Lq, Hq, D] over the states k, v [B, Lk, Hk, D] of another length (any strides over a
     contiguous D, so the halves of one key / value projection go in as views); Hq a multiple of Hk, query head h reads key head
     h // (Hq // Hk).  key_lens [B] int32: keys from key_lens[b] on are padding; key_mask [B, Lk] bool: False leaves a key out.
-    What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.
-    -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
+    What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.  D up to 256;
+    multiples of 8 run on the matrix cores (tensors whose rows do not start on 16 bytes are copied first), others on a plain kernel
+    that suits small calls.  -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
     dev = _gpu()
-    q, qs = _heads(_dev(q, "q", dev), "q")
+    q = _dev(q, "q", dev)
     code = _code(q, "q")
-    k, ks = _heads(_same_type(_dev(k, "k", dev), q, "k"), "k")
-    v, vs = _heads(_same_type(_dev(v, "v", dev), q, "v"), "v")
+    k, v = _same_type(_dev(k, "k", dev), q, "k"), _same_type(_dev(v, "v", dev), q, "v")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("cross_attention: q %s and k %s must be [B, L, H, D]" % (tuple(q.shape), tuple(k.shape)))
     B, Lq, Hq, D = q.shape
     Lk, Hk = k.shape[1:3]
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
         raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError("cross_attention: %d query heads over %d key heads of %d" % (Hq, Hk, D))
+    if D % 8 == 0:
+        q, k, v = _whole_rows(q), _whole_rows(k), _whole_rows(v)
+    (q, qs), (k, ks), (v, vs) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
     if key_lens is not None:
         key_lens = _dev(key_lens, "key_lens", dev)
         if tuple(key_lens.shape) != (B,) or key_lens.dtype not in (torch.int32, torch.int64):
@@ -373,7 +392,7 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
         key_mask = key_mask.contiguous()
     out = q.new_empty((B, Lq, Hq, D))
     L = _lib.lib()
-    need = L.yolo_cross_attention_workspace_bytes(code, B, Lq, Lk, Hq, Hk, D)
+    need = _attention_workspace(code, B, Lq, Lk, Hq, Hk, D)
     ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _lib.check(L.yolo_cross_attention(code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _tensor.ptr(key_lens),
                                       _tensor.ptr(key_mask), B, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None else float(scale),
