@@ -112,8 +112,8 @@ __device__ __forceinline__ u32x4 load_piece(const char* at, int k, int K) {
 // ALIGNED: rows of x and W start on 16 bytes and K is whole pieces; they go global -> LDS by DMA, pieces past K from a zero piece.
 // Otherwise the pieces pass through registers.
 //
-// Measured, bf16: 8192^3 1.27 PFLOP/s with 256 x 256 tiles of 16 waves (64 x 64 each, 113 registers, one workgroup a CU), 1.06 with
-// 128 x 128 (two a CU); the library's product reaches 1.08 on the same card.  23104 x 4096 x 1024 with gelu 0.86 PFLOP/s: six rounds of
+// Measured, bf16: 8192^3 1.31 PFLOP/s with 256 x 256 tiles of 16 waves (64 x 64 each, 116 registers, one workgroup a CU), 1.11 with
+// 128 x 128 (two a CU); the library's product reaches 1.08 on the same card.  23104 x 4096 x 1024 with gelu 0.87 PFLOP/s: six rounds of
 // 256 tiles, between which loads, stores and the activation are not covered by products.  173056 x 512 x 256 with gelu and residual
 // 3.3 TB/s, bandwidth and the same gaps.  Persistent workgroups that fetch the next tile before the epilogue were slower (128
 // registers do not hold both); f32 112 TFLOP/s at 23104 x 1024 x 512 (the f32 matrix peak is 157).
@@ -220,6 +220,15 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
 #pragma unroll
                 for (int j = 0; j < TM; ++j) acc[i][j] = mma<BF16>(fw[i], fx[j], acc[i][j]);
         }
+        // schedule: all fragments of the first half step, then those of the second between its products
+        constexpr int kReads = TM + TN, kProducts = TM * TN * (BF16 ? 1 : 4);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);                     // LDS reads
+#pragma unroll
+        for (int q = 0; q < kReads; ++q) {
+            __builtin_amdgcn_sched_group_barrier(0x8, kProducts / kReads, 0);       // MFMAs
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 2 * kProducts - kProducts / kReads * kReads, 0);
         if (s + 1 < nsteps) settle(buf ^ 1);
     }
 
@@ -448,7 +457,7 @@ static int launch_direct(LinK k, hipStream_t stream) {
 }
 
 // Tile by the time of a round of tiles on the 256 CUs, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU
-// takes 4, two 128 x 128 tiles 2.4 (1060 against 1260 TFLOP/s at 8192^3, twice the operand traffic), four 64 x 64 tiles 1.7.
+// takes 4, two 128 x 128 tiles 2.4 (1105 against 1309 TFLOP/s at 8192^3, twice the operand traffic), four 64 x 64 tiles 1.7.
 // Measured (bf16, us for 256 / 128 / 64): 23104 x 4096 x 1024 220 / 246 / 316, 10816 x 512 x 1024 31.7 / 22.3 / 26.9,
 // 2704 x 1024 x 512 42 / 12.4 / 9.6; f32 has no 256 x 256 (288 against 216 at 23104 x 1024 x 512: its registers do not fit).
 // Few outputs go to the direct kernel, which splits K inside a workgroup: up to 512 tiles of 16 x 16 (40 x 1024 x 1024: 4.1 against 6.7 in
