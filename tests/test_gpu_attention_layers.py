@@ -384,7 +384,7 @@ def test_attention_strides_and_alignment(L, t):
     assert (L.cross_attention(q, kv[:, :0, 0], kv[:, :0, 1]) == 0).all()
 
 
-def test_attention_deterministic_and_batch_independent(L):
+def test_attention_deterministic(L):
     for t in (BF16, F32):
         for lq in (1, 200):
             q, k, v = qkv(t, 3, lq, 1800, 8, 2, 64, 90)
@@ -626,3 +626,29 @@ def test_unaligned_attention_through_the_c_entry(L):
         u = torch.finfo(t).eps / 2
         a = L.cross_attention(q, k, v.abs(), key_lens=lens, key_mask=mask).double()
         within(out, want.double(), 2 * u * want.double().abs() + (2.0 ** -16 + (2 * u if t == BF16 else 0)) * 2 * a, t)
+
+
+def test_offsets_past_32_bits(L):
+    """Strides and sizes whose byte offsets pass 2^32: a state cache with far rows, wide rows of a matrix product, a result of more than
+    2^32 bytes."""
+    buf = torch.zeros(3_000_000_000, dtype=BF16, device="cuda")                    # 6 GB
+    far = buf.as_strided((1, 700, 2, 64), (0, 4_000_000, 64, 1))
+    q, k, v = qkv(BF16, 1, 5, 700, 4, 2, 64, 250)
+    far.copy_(k)
+    want = L.cross_attention(q, k, v)
+    assert torch.equal(L.cross_attention(q, far, v), want)
+    for lq in (1, 300):                                                            # one-wave and four-wave tiles
+        ql = rand((1, lq, 4, 64), BF16, 251)
+        assert torch.equal(L.cross_attention(ql, far, far), L.cross_attention(ql, k, k))
+    f, p = L.rope_frequencies(64), torch.arange(700, device="cuda")
+    assert torch.equal(L.qk_norm_rope(far, None, None, None, f, p)[0], L.qk_norm_rope(k, None, None, None, f, p)[0])
+    assert torch.equal(L.qk_norm_rope(far[..., :40], None)[0], L.qk_norm_rope(k[..., :40], None)[0])    # general kernel
+    x = far[0, :, 0]                                                               # rows 8 MB apart
+    w = rand((1000, 64), BF16, 252)
+    assert torch.equal(L.linear(x, w), L.linear(k[0, :, 0], w)) or torch.allclose(L.linear(x, w).float(), L.linear(k[0, :, 0], w).float(), rtol=2 ** -7, atol=2 ** -16)
+    del buf, far, x
+    x, w = rand((70_000, 16), BF16, 253), rand((32_768, 16), BF16, 254)
+    y = L.linear(x, w)                                                             # 4.6 GB
+    for rows in (slice(0, 64), slice(65_500, 65_600), slice(69_950, 70_000)):
+        check = x[rows].double().cpu() @ w.double().cpu().t()
+        assert ((y[rows].double().cpu() - check).abs() <= 2.0 ** -8 * check.abs() + 2.0 ** -18 * 64).all()
