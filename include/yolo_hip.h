@@ -232,9 +232,11 @@ int yolo2_nms(const double* boxes, const float* probs, int B, int n, int C, floa
 
 /* ---- attention-side layers (no counterpart in the reference): what a head needs in which cells, queries or prompts attend to
  * the maps of the networks above.  Inference only.  Element type float32 or bfloat16 (`dtype`: YOLO_DTYPE_*) for every
- * activation and weight matrix; arithmetic, sums and softmax in float32, one rounding at the store.  Outputs must not overlap
- * inputs; rows the outputs do not name are left as they were.  None allocates, synchronises or keeps anything between calls,
- * so calls may overlap on any streams and may be captured into a HIP graph. */
+ * activation and weight matrix; arithmetic, sums and softmax in float32, one rounding at the store (cross_attention in bfloat16 also
+ * rounds the weights of the values).  Outputs must not overlap inputs; memory the outputs do not name is left as it was.  None
+ * allocates, synchronises or keeps anything between calls, so calls may overlap on any streams (each with a workspace of its
+ * own) and may be captured into a HIP graph.  A call repeated gives the same bits; the kernel and the order of its sums go by the
+ * sizes of the call, so a row may differ in its last bits between calls of other batch sizes. */
 enum { YOLO_ACT_NONE = 0, YOLO_ACT_LEAKY = 1, YOLO_ACT_RELU = 2, YOLO_ACT_GELU = 3, YOLO_ACT_SILU = 4 };
 
 /* out[m,n] = act(sum_k x[m,k] * weight[n,k] + bias[n]) + residual[m,n]: the 1x1 conv2d of a feature map's cells (yolo_conv_forward)
@@ -250,8 +252,8 @@ int yolo_linear(int dtype, const void* x, int64_t x_ld, const void* weight, int6
  * position * frequencies[i]: pairs (i, i + rotary_dim/2), or (2i, 2i+1) if interleaved.  Queries and keys (of another length
  * and head count) in one launch; k = NULL: queries only (a step over keys that are normalised already).
  * q [B,Lq,Hq,D], k [B,Lk,Hk,D]: HOST *_strides = element strides of batch, token, head (last dimension contiguous);
- * q_out, k_out packed.  *_weight [D] of `weight_dtype`, or NULL (ones).  frequencies: DEVICE float64 [rotary_dim/2], radians per position, or NULL
- * (no rotation, positions unused).  *_positions: int32 (or int64: positions_int64) [L, axes], or [B, L, axes] if *_batched;
+ * q_out, k_out packed.  *_weight [D] of `weight_dtype`, or NULL (ones).  frequencies: DEVICE float64 [rotary_dim/2], radians per
+ * position (the angle is formed in float64), or NULL (no rotation, positions unused).  *_positions: int32 (or int64: positions_int64) [L, axes], or [B, L, axes] if *_batched;
  * with axes = 2 the first half of the pairs turns by coordinate 0, the second half by coordinate 1.  D <= 256, eps > 0. */
 int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const int64_t* q_strides, int Lq, int Hq, const void* q_weight,
                       const void* q_positions, void* q_out, const void* k, const int64_t* k_strides, int Lk, int Hk,
@@ -263,7 +265,10 @@ int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const int64_t* q_s
  * h / (Hq / Hk).  HOST *_strides as above, out [B,Lq,Hq,D] packed.  A key is kept when its index is below key_lens[b] (DEVICE int32
  * [B], NULL: Lk; values are clamped to [0, Lk]) and key_mask[b,j] (DEVICE uint8 [B,Lk], NULL: all) is not 0; other keys have no
  * influence whatever they hold.  A row without a kept key is zero (Lk = 0: all rows).  D <= 256, Hq a multiple of Hk.
- * D a multiple of 8 with 16-byte aligned rows takes the matrix-core kernels; any other head size, stride or alignment is accepted. */
+ * scale must be finite, Lk <= 2^30, B * Lq < 2^31.
+ * D a multiple of 8 with 16-byte aligned rows takes the matrix-core kernels; any other head size, stride or alignment is accepted
+ * by a plain kernel that suits small calls.  Few query rows over many keys split the keys over workgroups and join in a second launch:
+ * workspace (16-byte aligned) of yolo_cross_attention_workspace_bytes, 0 where none is needed or the arguments are refused. */
 size_t yolo_cross_attention_workspace_bytes(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D);
 int yolo_cross_attention(int dtype, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, const int32_t* key_lens, const uint8_t* key_mask, int B,

@@ -116,7 +116,7 @@ __device__ __forceinline__ u32x4 load_piece(const char* at, int k, int K) {
 // 128 x 128 (two a CU); the library's product reaches 1.08 on the same card.  23104 x 4096 x 1024 with gelu 0.87 PFLOP/s: six rounds of
 // 256 tiles, between which loads, stores and the activation are not covered by products.  173056 x 512 x 256 with gelu and residual
 // 3.3 TB/s, bandwidth and the same gaps.  Persistent workgroups that fetch the next tile before the epilogue were slower (128
-// registers do not hold both); f32 112 TFLOP/s at 23104 x 1024 x 512 (the f32 matrix peak is 157).
+// registers do not hold both); f32 117 TFLOP/s at 23104 x 1024 x 512 (the f32 matrix peak is 157).
 __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
 
 // Swaps lane rows so that a lane that holds 4 outputs of each of two 16-wide tiles (a: tile i, b: tile i + 1, packed pairs) holds 8
@@ -459,7 +459,7 @@ static int launch_direct(LinK k, hipStream_t stream) {
 // Tile by the time of a round of tiles on the 256 CUs, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU
 // takes 4, two 128 x 128 tiles 2.4 (1105 against 1309 TFLOP/s at 8192^3, twice the operand traffic), four 64 x 64 tiles 1.7.
 // Measured (bf16, us for 256 / 128 / 64): 23104 x 4096 x 1024 220 / 246 / 316, 10816 x 512 x 1024 31.7 / 22.3 / 26.9,
-// 2704 x 1024 x 512 42 / 12.4 / 9.6; f32 has no 256 x 256 (288 against 216 at 23104 x 1024 x 512: its registers do not fit).
+// 2704 x 1024 x 512 42 / 12.4 / 9.6; f32 has no 256 x 256 (288 against 207 at 23104 x 1024 x 512).
 // Few outputs go to the direct kernel, which splits K inside a workgroup: up to 512 tiles of 16 x 16 (40 x 1024 x 1024: 4.1 against 6.7 in
 // 32 x 32 and 8.2 in 64 x 64), up to 256 of 32 x 32 (300 x 512 x 1024: 7.4 against 11.2; 700 x 512 x 512, 352 tiles: 9.0 against 7.9), 512 in f32, whose products
 // take four times as long (300 x 512 x 1024: 10.8 against 24.6).
@@ -475,7 +475,12 @@ static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
     if constexpr (BF16) {
         if (aligned && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
     }
-    if (c128 <= c64) return aligned ? launch_tile<BF16, 128, 128, 2, 2, true>(k, stream) : launch_tile<BF16, 128, 128, 2, 2, false>(k, stream);
+    if (c128 <= c64) {
+        if (!aligned) return launch_tile<BF16, 128, 128, 2, 2, false>(k, stream);
+        // f32: sixteen waves of 32 x 32, 207 us against 215 with four of 64 x 64 at 23104 x 1024 x 512
+        if constexpr (!BF16) return launch_tile<BF16, 128, 128, 4, 4, true>(k, stream);
+        else return launch_tile<BF16, 128, 128, 2, 2, true>(k, stream);
+    }
     return aligned ? launch_tile<BF16, 64, 64, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 2, 2, false>(k, stream);
 }
 
