@@ -254,7 +254,8 @@ int yolo_linear(int dtype, const void* x, int64_t x_ld, const void* weight, int6
  * q [B,Lq,Hq,D], k [B,Lk,Hk,D]: HOST *_strides = element strides of batch, token, head (last dimension contiguous);
  * q_out, k_out packed.  *_weight [D] of `weight_dtype`, or NULL (ones).  frequencies: DEVICE float64 [rotary_dim/2], radians per
  * position (the angle is formed in float64), or NULL (no rotation, positions unused).  *_positions: int32 (or int64: positions_int64) [L, axes], or [B, L, axes] if *_batched;
- * with axes = 2 the first half of the pairs turns by coordinate 0, the second half by coordinate 1.  D <= 256, eps > 0. */
+ * with axes = 2 the first half of the pairs turns by coordinate 0, the second half by coordinate 1.  D <= 256, eps > 0; the sum of
+ * squares is float32 (elements up to about 10^18). */
 int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const int64_t* q_strides, int Lq, int Hq, const void* q_weight,
                       const void* q_positions, void* q_out, const void* k, const int64_t* k_strides, int Lk, int Hk,
                       const void* k_weight, const void* k_positions, void* k_out, int weight_dtype, const double* frequencies,

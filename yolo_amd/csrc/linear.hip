@@ -28,11 +28,11 @@ struct LinK {
 // Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7; a bf16 half step is 2^-8 of the value).  One reciprocal, one exponential and
 // eleven other instructions against about forty and a divergent branch: at 23104 x 4096 results the difference is a
 // quarter of the whole product's time.  The factor 1/2 is in the coefficients; |v| is cut at 16, where the exponential is 0, so that
-// +inf stays +inf.
+// +inf stays +inf and -inf gives 0.
 template <bool BF16>
 __device__ __forceinline__ float gelu(float v) {
     if constexpr (!BF16) {
-        return 0.5f * v * erfcf(-0.70710678118654752f * v);
+        return v < -14.5f ? 0.f : 0.5f * v * erfcf(-0.70710678118654752f * v);      // 0 from there on, also at -inf
     } else {
         const float a = __builtin_fabsf(v);
         const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, a, 1.0f));
