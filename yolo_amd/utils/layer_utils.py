@@ -273,12 +273,14 @@ def _heads(x, name):
     return x, _Strides(st[0], st[1], st[2])
 
 
-def _whole_rows(x):
-    """x [B, L, H, D] itself if all its rows start on 16 bytes, which the matrix-core kernels need, else a copy."""
-    st, z = x.stride(), x.element_size()
-    if (x.data_ptr() | st[0] * z | st[1] * z | st[2] * z) & 15:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+def _attention_operand(x, D):
+    """[B, L, H, D] -> (tensor, ctypes strides of batch, token, head); copied if D is not contiguous or, where the matrix-core kernels
+    could run (D a multiple of 8), if a row does not start on 16 bytes."""
+    st = x.stride()
+    if (st[3] != 1 and D > 1) or (D % 8 == 0 and (x.data_ptr() | (st[0] | st[1] | st[2]) * x.element_size()) & 15):
+        x = x.clone(memory_format=torch.contiguous_format)
+        st = x.stride()
+    return x, _Strides(st[0], st[1], st[2])
 
 
 def _positions(p, B, L, axes, name, dev):
@@ -375,9 +377,7 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
         raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError("cross_attention: %d query heads over %d key heads of %d" % (Hq, Hk, D))
-    if D % 8 == 0:
-        q, k, v = _whole_rows(q), _whole_rows(k), _whole_rows(v)
-    (q, qs), (k, ks), (v, vs) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    (q, qs), (k, ks), (v, vs) = _attention_operand(q, D), _attention_operand(k, D), _attention_operand(v, D)
     if key_lens is not None:
         key_lens = _dev(key_lens, "key_lens", dev)
         if tuple(key_lens.shape) != (B,) or key_lens.dtype not in (torch.int32, torch.int64):
