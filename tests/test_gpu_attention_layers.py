@@ -652,3 +652,29 @@ def test_offsets_past_32_bits(L):
     for rows in (slice(0, 64), slice(65_500, 65_600), slice(69_950, 70_000)):
         check = x[rows].double().cpu() @ w.double().cpu().t()
         assert ((y[rows].double().cpu() - check).abs() <= 2.0 ** -8 * check.abs() + 2.0 ** -18 * 64).all()
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("d", [1, 7, 20, 63, 100, 255])
+def test_attention_odd_head_sizes_through_the_c_entry(L, t, d):
+    """Any head size straight into the C entry (the Python function pads it): the general kernel, with lens and a mask."""
+    import ctypes
+    from yolo_amd import _lib, _tensor
+    q, k, v = qkv(t, 2, 5, 130, 4, 2, d, 260)
+    lens = torch.tensor([130, 67], dtype=torch.int32, device="cuda")
+    mask = torch.ones((2, 130), dtype=torch.bool, device="cuda")
+    mask[1, ::5] = False
+    st = [(ctypes.c_int64 * 3)(*x.stride()[:3]) for x in (q, k, v)]
+    assert _lib.lib().yolo_cross_attention_workspace_bytes(0, 2, 5, 130, 4, 2, d) == 0
+
+    def call(q, k, v, key_lens, key_mask, scale):
+        out = torch.full((2, 5, 4, d), 9.0, dtype=t, device="cuda")
+        _lib.check(_lib.lib().yolo_cross_attention(0 if t == F32 else 1, q.data_ptr(), st[0], k.data_ptr(), st[1], v.data_ptr(), st[2],
+                                                   key_lens.data_ptr(), key_mask.data_ptr(), 2, 5, 130, 4, 2, d, d ** -0.5, out.data_ptr(), None, 0,
+                                                   _tensor.stream_ptr()))
+        return out
+
+    class Entry:
+        cross_attention = staticmethod(call)
+    check_attention(Entry, q, k, v, lens, mask, what=("c entry", d))
+    check_attention(L, q, k, v, lens, mask, what=("padded", d))

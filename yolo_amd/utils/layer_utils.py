@@ -363,8 +363,8 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     contiguous D, so the halves of one key / value projection go in as views); Hq a multiple of Hk, query head h reads key head
     h // (Hq // Hk).  key_lens [B] int32: keys from key_lens[b] on are padding; key_mask [B, Lk] bool: False leaves a key out.
     What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.  D up to 256;
-    multiples of 8 run on the matrix cores (tensors whose rows do not start on 16 bytes are copied first), others on a plain kernel
-    that suits small calls.  -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
+    tensors whose rows do not start on 16 bytes are copied first, head sizes that are not multiples of 8 padded.
+    -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
     dev = _gpu()
     q = _dev(q, "q", dev)
     code = _code(q, "q")
@@ -377,6 +377,12 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
         raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
         raise ValueError("cross_attention: %d query heads over %d key heads of %d" % (Hq, Hk, D))
+    if scale is None:
+        scale = D ** -0.5
+    if D % 8 and D <= 256 and Lk:
+        # zeros up to the next multiple of 8 change no score and add no result: copies, but on the matrix cores
+        pad = (0, -D % 8)
+        return cross_attention(*[torch.nn.functional.pad(x, pad) for x in (q, k, v)], key_lens, key_mask, scale)[..., :D].contiguous()
     (q, qs), (k, ks), (v, vs) = _attention_operand(q, D), _attention_operand(k, D), _attention_operand(v, D)
     if key_lens is not None:
         key_lens = _dev(key_lens, "key_lens", dev)
@@ -395,6 +401,6 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     need = _attention_workspace(code, B, Lq, Lk, Hq, Hk, D)
     ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     _lib.check(L.yolo_cross_attention(code, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, _tensor.ptr(key_lens),
-                                      _tensor.ptr(key_mask), B, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None else float(scale),
+                                      _tensor.ptr(key_mask), B, Lq, Lk, Hq, Hk, D, float(scale),
                                       out.data_ptr(), _tensor.ptr(ws), need, _tensor.stream_ptr(dev)))
     return out
