@@ -75,6 +75,14 @@ def test_linear_sizes(L, t, m, k, n, act, bias, res):
 
 
 @pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("m,k,n", [(16833, 64, 32), (17000, 72, 31), (20001, 33, 17), (33000, 20, 1)])
+@pytest.mark.parametrize("act,bias,res", [(None, False, False), ("silu", True, True)])
+def test_linear_narrow_outputs(L, t, m, k, n, act, bias, res):
+    x, w = rand((m, k), t, 1), rand((n, k), t, 2, k ** -0.5)
+    check_linear(L, x, w, rand((n,), t, 3) if bias else None, act, rand((m, n), t, 4) if res else None, (t, m, k, n))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("m", [5, 2100])
 def test_linear_activations(L, t, act, m):

@@ -463,6 +463,8 @@ static int launch_direct(LinK k, hipStream_t stream) {
 // Few outputs go to the direct kernel, which splits K inside a workgroup: up to 512 tiles of 16 x 16 (40 x 1024 x 1024: 4.1 against 6.7 in
 // 32 x 32 and 8.2 in 64 x 64), up to 256 of 32 x 32 (300 x 512 x 1024: 7.4 against 11.2; 700 x 512 x 512, 352 tiles: 9.0 against 7.9), 512 in f32, whose products
 // take four times as long (300 x 512 x 1024: 10.8 against 24.6).
+// Up to 32 columns take tiles of 64 x 32, as a wider one multiplies rows of W that are not there: 57289 x 32 x 1008 in f32 55 us (4.3 TB/s)
+// against 83 with 64 x 64, in bf16 31 against 34; 100000 x 32 x 64 in bf16 7.3 against 8.2.
 // The direct kernel forms 64-bit addresses; the tile kernel offsets rows of a tile in 32 bits and takes strides up to 4 MB.
 template <bool BF16>
 static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
@@ -471,6 +473,7 @@ static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
     const bool wide = k.x_ld > kMaxStride || k.w_ld > kMaxStride || k.out_ld > kMaxStride || (k.res && k.res_ld > kMaxStride);
     if (tiles(16) <= 512) return aligned ? launch_direct<BF16, 1, 1, true>(k, stream) : launch_direct<BF16, 1, 1, false>(k, stream);
     if (tiles(32) <= (BF16 ? 256 : 512) || wide) return aligned ? launch_direct<BF16, 2, 2, true>(k, stream) : launch_direct<BF16, 2, 2, false>(k, stream);
+    if (k.N <= 32) return aligned ? launch_tile<BF16, 64, 32, 4, 1, true>(k, stream) : launch_tile<BF16, 64, 32, 4, 1, false>(k, stream);
     const double c256 = (double)((tiles(256) + 255) / 256) * 4.0, c128 = (double)((tiles(128) + 511) / 512) * 2.4, c64 = (double)((tiles(64) + 1023) / 1024) * 1.7;
     if constexpr (BF16) {
         if (aligned && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
