@@ -266,7 +266,8 @@ int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const int64_t* q_s
  * h / (Hq / Hk).  HOST *_strides as above, out [B,Lq,Hq,D] packed.  A key is kept when its index is below key_lens[b] (DEVICE int32
  * [B], NULL: Lk; values are clamped to [0, Lk]) and key_mask[b,j] (DEVICE uint8 [B,Lk], NULL: all) is not 0; other keys have no
  * influence whatever they hold.  A row without a kept key is zero (Lk = 0: all rows).  D <= 256, Hq a multiple of Hk.
- * scale must be finite, Lk <= 2^30, B * Lq < 2^31.
+ * scale must be finite, Lk <= 2^30, B * Lq < 2^31.  Weighted values are summed in float32 before the division, with weights up to 2^8: |v| * Lk
+ * up to about 10^36.
  * D a multiple of 8 with 16-byte aligned rows takes the matrix-core kernels; any other head size, stride or alignment is accepted
  * by a plain kernel that suits small calls.  Few query rows over many keys split the keys over workgroups and join in a second launch:
  * workspace (16-byte aligned) of yolo_cross_attention_workspace_bytes, 0 where none is needed or the arguments are refused. */

@@ -351,6 +351,27 @@ def test_attention_scales_and_extreme_scores(L, t):
     check_attention(L, (q * 0 + 8), (k * 0 + 20), v, scale=1.0, what=("constant",))
 
 
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("lq,lk,d", [(50, 333, 64), (1, 2000, 32), (300, 700, 128), (7, 90, 5)])
+@pytest.mark.parametrize("size", [2.0 ** 12, 2.0 ** 15, 2.0 ** 40])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_huge_scores_select_the_largest(L, t, lq, lk, d, size, sign):
+    """Scores size^2 * (whole number up to 13) * 0.3, exact before the scale, whose distances are far beyond the range of exp: the
+    weights are 1 and 0, so a row is the value of its one largest key (the last, or the second), to one rounding of the quotient."""
+    q, k, v = torch.zeros(1, lq, 2, d), torch.zeros(1, lk, 2, d), torch.randn(1, lk, 2, d, generator=torch.Generator().manual_seed(5))
+    q[..., 0] = size
+    k[..., 0] = size * (torch.arange(lk) % 11).float()[None, :, None]
+    k[0, -1, 0, 0], k[0, 1, 1, 0] = 12 * size, 13 * size
+    if sign < 0:
+        k = -k
+    q, k, v = q.to(t).cuda(), k.to(t).cuda(), v.to(t).cuda()
+    got = L.cross_attention(q, k, v, scale=0.3 * sign)
+    want = torch.stack([v[0, -1, 0], v[0, 1, 1]])[None, None].expand(1, lq, 2, d)
+    # exp(0) and the sum are 1 up to the 2^-20 of the exponential's error: the quotient is off by that and the rounding
+    bound = want.double().abs() * (2.0 ** -20 + torch.finfo(t).eps / 2)
+    within(got, want.double(), bound, (t, lq, lk, d, size, sign))
+
+
 def test_attention_infinite_scores_follow_the_formula(L):
     """+inf among the kept scores: inf - inf makes the row NaN; -inf: weight zero; all -inf: NaN; other rows untouched."""
     for t in (BF16, F32):

@@ -303,7 +303,17 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[i][r] *= c;
         }
-        const float base = mref == -__builtin_inff() ? 0.f : mref * p.scale2;
+        // the rounding of `base` is a factor common to the row's weights, 2^(2^-24 base): past 4096 the maximum is subtracted first, as the
+        // factor would overflow from 2^31 on
+        float base = mref == -__builtin_inff() ? 0.f : mref * p.scale2;
+        if (__any(fabsf(base) > 4096.f)) {
+            const float mx = base == 0.f ? 0.f : mref;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[kb][r] -= mx;
+            base = 0.f;
+        }
         float st = 0.f;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
