@@ -83,6 +83,18 @@ def test_linear_narrow_outputs(L, t, m, k, n, act, bias, res):
 
 
 @pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("m,n", [(20, 40), (300, 80), (1500, 300), (9000, 20), (4100, 1100)])
+@pytest.mark.parametrize("k", [1, 3, 7, 9, 61, 65, 127, 263])
+def test_linear_rows_that_end_inside_a_piece(L, t, m, n, k):
+    """Unaligned rows inside a larger matrix of NaN: nothing outside a row has influence, wherever its last 16 bytes start."""
+    big_x, big_w = torch.full((m, k + 7), float("nan"), dtype=t, device="cuda"), torch.full((n, k + 5), float("nan"), dtype=t, device="cuda")
+    x, w = big_x[:, 3:3 + k], big_w[:, 2:2 + k]
+    x.copy_(rand((m, k), t, 1))
+    w.copy_(rand((n, k), t, 2, k ** -0.5))
+    check_linear(L, x, w, rand((n,), t, 3), None, None, (t, m, k, n))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("m", [5, 2100])
 def test_linear_activations(L, t, act, m):

@@ -83,24 +83,35 @@ __device__ __forceinline__ f32x4 mma(u32x4 a, u32x4 b, f32x4 c) {
     }
 }
 
-// The 16-byte piece at `at`, which is element k of its row, elements past K as zeros.  Rows need no alignment beyond their element's:
-// a whole piece is one load (global memory takes any address), the last one goes element by element.
-template <bool BF16>
+// A piece of an unaligned row: element k is at `at`.  The 16 bytes from element k on (global memory takes any address), or, where they
+// would pass the row's end, the row's last 16 bytes; of a row of less than 16 bytes (SHORT) its elements, with zeros before them.
+template <bool BF16, bool SHORT>
 __device__ __forceinline__ u32x4 load_piece(const char* at, int k, int K) {
     typedef typename Elem<BF16>::type T;
     constexpr int P = Elem<BF16>::kPiece;
-    u32x4 v = {0, 0, 0, 0};
-    const T* p = (const T*)at;
-    if (k + P <= K) {
-        __builtin_memcpy(&v, p, 16);
-    } else {
+    const T* p = (const T*)at + min(0, K - P - k);
+    if constexpr (SHORT) {
         typename std::conditional<BF16, bf16x8, f32x4>::type e = {};
 #pragma unroll
         for (int j = 0; j < P; ++j)
-            if (k + j < K) e[j] = p[j];
-        v = __builtin_bit_cast(u32x4, e);
+            if (j >= P - K) e[j] = p[j];
+        return __builtin_bit_cast(u32x4, e);
+    } else {
+        u32x4 v;
+        __builtin_memcpy(&v, p, 16);
+        return v;
     }
-    return v;
+}
+
+// What load_piece read, as the piece of element k: moved down to its place, zeros past K.  One by one, the end's elements cost 2 us of 9 where
+// the chain is short (1001 x 255 x 255).
+template <bool BF16>
+__device__ __forceinline__ u32x4 place_piece(u32x4 v, int k, int K) {
+    constexpr int P = Elem<BF16>::kPiece, Z = 16 / P;
+    const int excess = k + P - K;
+    if (excess <= 0) return v;
+    if (excess >= P) return u32x4{0, 0, 0, 0};
+    return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (excess * Z * 8));
 }
 
 // ---- tiles of BM rows of x by BN rows of W through LDS ------------------------------------------------------------------------
@@ -177,12 +188,24 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
                     dma16(s * BK + kc < p.K ? (const void*)((i < LX ? xs : ws) + off[i]) : (const void*)&kZeroPiece, dst + i * NT * 16);
             }
         } else {
+            if ((s + 1) * BK <= p.K) {
 #pragma unroll
-            for (int i = 0; i < LX + LW; ++i) stage[i] = load_piece<BF16>((i < LX ? xs : ws) + off[i], s * BK + kc, p.K);
+                for (int i = 0; i < LX + LW; ++i) __builtin_memcpy(&stage[i], (i < LX ? xs : ws) + off[i], 16);
+            } else if (p.K >= P) {
+#pragma unroll
+                for (int i = 0; i < LX + LW; ++i) stage[i] = load_piece<BF16, false>((i < LX ? xs : ws) + off[i], s * BK + kc, p.K);
+            } else {
+#pragma unroll
+                for (int i = 0; i < LX + LW; ++i) stage[i] = load_piece<BF16, true>((i < LX ? xs : ws) + off[i], s * BK + kc, p.K);
+            }
         }
     };
-    auto settle = [&](int buf) {                            // not ALIGNED: registers -> LDS
+    auto settle = [&](int s, int buf) {                     // not ALIGNED: registers -> LDS
         if constexpr (!ALIGNED) {
+            if ((s + 1) * BK > p.K) {
+#pragma unroll
+                for (int i = 0; i < LX + LW; ++i) stage[i] = place_piece<BF16>(stage[i], s * BK + kc, p.K);
+            }
 #pragma unroll
             for (int i = 0; i < LX + LW; ++i) *(u32x4*)(lds + buf * BUF + (i * NT + tid) * 16) = stage[i];
         }
@@ -199,7 +222,7 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = bv;
     }
-    settle(0);
+    settle(0, 0);
     for (int s = 0; s < nsteps; ++s) {
         const int buf = s & 1;
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -229,7 +252,7 @@ __global__ __launch_bounds__(WR* WC * 64, lin_blocks(BM, BN) * WR * WC / 4) void
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
         __builtin_amdgcn_sched_group_barrier(0x8, 2 * kProducts - kProducts / kReads * kReads, 0);
-        if (s + 1 < nsteps) settle(buf ^ 1);
+        if (s + 1 < nsteps) settle(s + 1, buf ^ 1);
     }
 
     // epilogue in registers: lane holds y[m][n .. n+3] for m = wm0 + 16 j + fr, n = wn0 + 16 i + 4 fh.  Results leave and residuals come in
@@ -354,53 +377,63 @@ __global__ __launch_bounds__(512) void linear_direct_kernel(LinK p) {
     typedef typename Elem<BF16>::type T;
     constexpr int W = 8, P = Elem<BF16>::kPiece, BK = 4 * P, BM = TM * 16, BN = TN * 16;
     __shared__ float part[W][BM * BN];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned tile = xcd_chunk(blockIdx.x, p.ntm * p.ntn);
     const unsigned tm = tile % p.ntm, tn = tile / p.ntm;     // row tiles of one W tile next to each other
     const long long m0 = (long long)tm * BM;
     const int n0 = (int)tn * BN;
     const int fr = lane & 15, fh = lane >> 4;
     const int nslices = (p.K + BK - 1) / BK;
+    // rows past the last one read the last one again: their results are not stored
     const char* xr[TM];
     const char* wr[TN];
 #pragma unroll
-    for (int j = 0; j < TM; ++j) {
-        const long long m = m0 + j * 16 + fr;
-        xr[j] = m < p.M ? p.x + m * p.x_ld : nullptr;
-    }
+    for (int j = 0; j < TM; ++j) xr[j] = p.x + min(m0 + j * 16 + fr, p.M - 1) * p.x_ld;
 #pragma unroll
-    for (int i = 0; i < TN; ++i) {
-        const int n = n0 + i * 16 + fr;
-        wr[i] = n < p.N ? p.w + (long long)n * p.w_ld : nullptr;
-    }
+    for (int i = 0; i < TN; ++i) wr[i] = p.w + (long long)min(n0 + i * 16 + fr, p.N - 1) * p.w_ld;
     f32x4 acc[TN][TM];
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int j = 0; j < TM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto piece = [&](const char* row, int k) {
-        const bool in = row != nullptr && k < p.K;
-        if constexpr (ALIGNED) return *(in ? (const u32x4*)(row + (long long)k * sizeof(T)) : &kZeroPiece);
-        else return in ? load_piece<BF16>(row + (long long)k * sizeof(T), k, p.K) : u32x4{0, 0, 0, 0};
-    };
-    constexpr int U = 4;                                     // slices in flight; those past K read zeros
-    for (int s = wave; s < nslices; s += U * W) {
-        u32x4 fx[U][TM], fw[U][TN];
+    constexpr int U = 4;                                     // slices in flight; those past K are zeros
+    auto walk = [&](auto is_short) {
+        auto piece = [&](const char* row, int k) {
+            if constexpr (ALIGNED) return *(k < p.K ? (const u32x4*)(row + (long long)k * sizeof(T)) : &kZeroPiece);
+            else return load_piece<BF16, decltype(is_short)::value>(row + (long long)k * sizeof(T), k, p.K);
+        };
+        for (int s = wave; s < nslices; s += U * W) {
+            u32x4 fx[U][TM], fw[U][TN];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = (s + u * W) * BK + fh * P;
+            for (int u = 0; u < U; ++u) {
+                const int k = (s + u * W) * BK + fh * P;
+                if (!ALIGNED && s + u * W >= nslices) break;
 #pragma unroll
-            for (int i = 0; i < TN; ++i) fw[u][i] = piece(wr[i], k);
+                for (int i = 0; i < TN; ++i) fw[u][i] = piece(wr[i], k);
 #pragma unroll
-            for (int j = 0; j < TM; ++j) fx[u][j] = piece(xr[j], k);
+                for (int j = 0; j < TM; ++j) fx[u][j] = piece(xr[j], k);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int k0 = (s + u * W) * BK;
+                if constexpr (!ALIGNED) {
+                    if (s + u * W >= nslices) break;
+                    if (k0 + BK > p.K) {
+#pragma unroll
+                        for (int i = 0; i < TN; ++i) fw[u][i] = place_piece<BF16>(fw[u][i], k0 + fh * P, p.K);
+#pragma unroll
+                        for (int j = 0; j < TM; ++j) fx[u][j] = place_piece<BF16>(fx[u][j], k0 + fh * P, p.K);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TN; ++i)
+#pragma unroll
+                    for (int j = 0; j < TM; ++j) acc[i][j] = mma<BF16>(fw[u][i], fx[u][j], acc[i][j]);
+            }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-                for (int j = 0; j < TM; ++j) acc[i][j] = mma<BF16>(fw[u][i], fx[u][j], acc[i][j]);
-    }
+    };
+    if (ALIGNED || p.K >= P) walk(std::false_type{});
+    else walk(std::true_type{});
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
@@ -479,12 +512,13 @@ static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
         if (aligned && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
     }
     if (c128 <= c64) {
-        if (!aligned) return launch_tile<BF16, 128, 128, 2, 2, false>(k, stream);
-        // f32: sixteen waves of 32 x 32, 207 us against 215 with four of 64 x 64 at 23104 x 1024 x 512
+        // sixteen waves of 32 x 32 in f32, 207 us against 215 with four of 64 x 64 at 23104 x 1024 x 512, and where pieces pass through registers,
+        // 100 against 103 at 23104 x 1024 x 1023; 64 x 64 unaligned likewise 7.1 against 8.1 at 1001 x 255 x 255
+        if (!aligned) return launch_tile<BF16, 128, 128, 4, 4, false>(k, stream);
         if constexpr (!BF16) return launch_tile<BF16, 128, 128, 4, 4, true>(k, stream);
         else return launch_tile<BF16, 128, 128, 2, 2, true>(k, stream);
     }
-    return aligned ? launch_tile<BF16, 64, 64, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 2, 2, false>(k, stream);
+    return aligned ? launch_tile<BF16, 64, 64, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 4, 2, false>(k, stream);
 }
 
 }  // namespace yolo
