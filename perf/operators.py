@@ -185,7 +185,7 @@ def run(s):
             return L.linear(s["x"], s["w"], s["b"], activation=s["activation"], residual=s["r"])
         if s["op"] == "qk":
             q, k = L.qk_norm_rope(s["q"], s["k"], s["qw"], s["kw"], frequencies=s["f"], q_positions=s["qp"], k_positions=s["kp"],
-                                  eps=1e-6, interleaved=s["interleaved"])
+                                  eps=1e-6, interleaved=s["interleaved"], axes=s["qp"].dim())
             return (q,) if k is None else (q, k)
         return L.cross_attention(s["q"], s["kv"][:, :, 0], s["kv"][:, :, 1], key_lens=s["lens"], key_mask=s["mask_keys"])
     if s["op"] == "linear":
