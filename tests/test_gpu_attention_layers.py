@@ -95,6 +95,16 @@ def test_linear_rows_that_end_inside_a_piece(L, t, m, n, k):
 
 
 @pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("m,k,n", [(12300, 64, 640), (12301, 136, 648), (12289, 72, 641), (2800, 512, 2056), (6001, 264, 1100), (1537, 200, 1030),
+                                   (20000, 96, 96), (9500, 320, 130), (30000, 24, 250), (4160, 1000, 520)])
+@pytest.mark.parametrize("act,bias,res", [(None, False, False), ("gelu", True, True)])
+def test_linear_tile_shapes(L, t, m, k, n, act, bias, res):
+    """Sizes on either side of every choice of a tile, whole and ragged in both directions."""
+    x, w = rand((m, k), t, 1), rand((n, k), t, 2, k ** -0.5)
+    check_linear(L, x, w, rand((n,), t, 3) if bias else None, act, rand((m, n), t, 4) if res else None, (t, m, k, n))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
 @pytest.mark.parametrize("act", list(ACTS))
 @pytest.mark.parametrize("m", [5, 2100])
 def test_linear_activations(L, t, act, m):

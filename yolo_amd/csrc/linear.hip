@@ -489,10 +489,14 @@ static int launch_direct(LinK k, hipStream_t stream) {
     return YOLO_OK;
 }
 
-// Tile by the time of a round of tiles on the 256 CUs, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU
-// takes 4, two 128 x 128 tiles 2.4 (1105 against 1309 TFLOP/s at 8192^3, twice the operand traffic), four 64 x 64 tiles 1.7.
-// Measured (bf16, us for 256 / 128 / 64): 23104 x 4096 x 1024 220 / 246 / 316, 10816 x 512 x 1024 31.7 / 22.3 / 26.9,
-// 2704 x 1024 x 512 42 / 12.4 / 9.6; f32 has no 256 x 256 (288 against 207 at 23104 x 1024 x 512).
+// Tile by the time that the rounds of its tiles on the 256 CUs take.
+// bf16, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU takes 4 (1309 TFLOP/s at 8192^3, 128 x 128 1105 with twice the
+// operand traffic), two of 192 x 128 3.35, two of 128 x 128 2.55, four of 64 x 64 1.75: fitted to 67 shapes (600 to 200000 rows, 48 to 8192
+// wide), where the choice is 2 % from the best of six tiles on average.  Measured (us for 256 / 192 / 128 / 64): 23104 x 4096 x 1024 217 / 227 /
+// 244 / 319, 5000 x 2048 x 2048 55 / 45 / 58 / 69, 8000 x 1024 x 1024 30 / 26 / 23 / 34, 2704 x 1024 x 256 15.5 / 9.4 / 8.8 / 6.9.
+// f32 is bound by its products: rounds of one tile a CU times the tile, 96 x 64 counted 2 % and 128 x 128 4 % cheaper for their fewer operand reads.
+// Measured (us for 128 / 96 / 64): 23104 x 1024 x 512 207 / 210 / 212, 5408 x 512 x 512 39 / 32 / 35, 1500 x 1024 x 1024 69 / 32 / 40,
+// 2194 x 864 x 1680 114 / 89 / 64; within 1.2 % of the best of six tiles on average over 44 of the shapes.
 // Few outputs go to the direct kernel, which splits K inside a workgroup: up to 512 tiles of 16 x 16 (40 x 1024 x 1024: 4.1 against 6.7 in
 // 32 x 32 and 8.2 in 64 x 64), up to 256 of 32 x 32 (300 x 512 x 1024: 7.4 against 11.2; 700 x 512 x 512, 352 tiles: 9.0 against 7.9), 512 in f32, whose products
 // take four times as long (300 x 512 x 1024: 10.8 against 24.6).
@@ -507,18 +511,26 @@ static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
     if (tiles(16) <= 512) return aligned ? launch_direct<BF16, 1, 1, true>(k, stream) : launch_direct<BF16, 1, 1, false>(k, stream);
     if (tiles(32) <= (BF16 ? 256 : 512) || wide) return aligned ? launch_direct<BF16, 2, 2, true>(k, stream) : launch_direct<BF16, 2, 2, false>(k, stream);
     if (k.N <= 32) return aligned ? launch_tile<BF16, 64, 32, 4, 1, true>(k, stream) : launch_tile<BF16, 64, 32, 4, 1, false>(k, stream);
-    const double c256 = (double)((tiles(256) + 255) / 256) * 4.0, c128 = (double)((tiles(128) + 511) / 512) * 2.4, c64 = (double)((tiles(64) + 1023) / 1024) * 1.7;
+    auto rounds = [&](int bm, int bn, int slots) {
+        const unsigned long long n = (unsigned long long)((k.M + bm - 1) / bm) * ((k.N + bn - 1) / bn);
+        return (double)((n + slots - 1) / slots);
+    };
+    // where pieces pass through registers, sixteen waves of 32 x 32 take 100 us against 103 with four of 64 x 64 at 23104 x 1024 x 1023, and
+    // eight of 16 x 32 7.1 against 8.1 with four of 32 x 32 at 1001 x 255 x 255; in f32 likewise 207 against 215 at 23104 x 1024 x 512 and 35 against 37
+    // at 5408 x 512 x 512
     if constexpr (BF16) {
-        if (aligned && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
+        const double c256 = rounds(256, 256, 256) * 4.0, c192 = rounds(192, 128, 512) * 3.35, c128 = rounds(128, 128, 512) * 2.55;
+        const double c64 = rounds(64, 64, 1024) * 1.75;
+        if (!aligned) return c128 <= c64 ? launch_tile<BF16, 128, 128, 4, 4, false>(k, stream) : launch_tile<BF16, 64, 64, 4, 2, false>(k, stream);
+        if (c256 <= c192 && c256 <= c128 && c256 <= c64) return launch_tile<BF16, 256, 256, 4, 4, true>(k, stream);
+        if (c192 <= c128 && c192 <= c64) return launch_tile<BF16, 192, 128, 4, 2, true>(k, stream);
+        return c128 <= c64 ? launch_tile<BF16, 128, 128, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 2, 2, true>(k, stream);
+    } else {
+        const double c128 = rounds(128, 128, 256) * 4.0 * 0.96, c96 = rounds(96, 64, 256) * 1.5 * 0.98, c64 = rounds(64, 64, 256);
+        if (!aligned) return c128 <= c64 ? launch_tile<BF16, 128, 128, 4, 4, false>(k, stream) : launch_tile<BF16, 64, 64, 4, 2, false>(k, stream);
+        if (c128 <= c96 && c128 <= c64) return launch_tile<BF16, 128, 128, 4, 4, true>(k, stream);
+        return c96 <= c64 ? launch_tile<BF16, 96, 64, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 4, 2, true>(k, stream);
     }
-    if (c128 <= c64) {
-        // sixteen waves of 32 x 32 in f32, 207 us against 215 with four of 64 x 64 at 23104 x 1024 x 512, and where pieces pass through registers,
-        // 100 against 103 at 23104 x 1024 x 1023; 64 x 64 unaligned likewise 7.1 against 8.1 at 1001 x 255 x 255
-        if (!aligned) return launch_tile<BF16, 128, 128, 4, 4, false>(k, stream);
-        if constexpr (!BF16) return launch_tile<BF16, 128, 128, 4, 4, true>(k, stream);
-        else return launch_tile<BF16, 128, 128, 2, 2, true>(k, stream);
-    }
-    return aligned ? launch_tile<BF16, 64, 64, 2, 2, true>(k, stream) : launch_tile<BF16, 64, 64, 4, 2, false>(k, stream);
 }
 
 }  // namespace yolo
