@@ -358,6 +358,26 @@ def test_attention_masks(L, t, lq, lk):
 
 
 @pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("d", [136, 160, 192, 248, 256])
+@pytest.mark.parametrize("b,lq,lk,hq,hk", [(1, 1, 1, 1, 1), (2, 3, 40, 4, 2), (1, 200, 33, 2, 2), (3, 33, 700, 4, 1), (4, 700, 100, 4, 4)])
+def test_attention_wide_heads(L, t, d, b, lq, lk, hq, hk):
+    """Head sizes whose values are divided over workgroups, with and without key splits; masked keys hold NaN."""
+    q, k, v = qkv(t, b, lq, lk, hq, hk, d, 71)
+    check_attention(L, q, k, v, what=(t, d, b, lq, lk))
+    keep = torch.rand(b, lk, generator=torch.Generator().manual_seed(4)) < 0.7
+    keep[0] = False
+    keep = keep.cuda()
+    k[~keep] = float("nan")
+    v[~keep] = float("nan")
+    got = L.cross_attention(q, k, v, key_mask=keep)
+    assert torch.isfinite(got).all() and not got[0].any()
+    k[~keep] = 0
+    v[~keep] = 0
+    assert torch.equal(got, L.cross_attention(q, k, v, key_mask=keep))
+    check_attention(L, q, k, v, mask=keep, what=("mask", t, d, b, lq, lk))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
 def test_attention_scales_and_extreme_scores(L, t):
     q, k, v = qkv(t, 2, 50, 333, 4, 4, 64, 60)
     for scale in (0.0, -0.2, 1.0, 3.0):

@@ -123,6 +123,11 @@ __global__ __launch_bounds__(256) void cross_attention_general_kernel(AttnK p) {
 // bf16: the weights are rounded to bf16 for the second product, at most 2^-8 of each and of either sign, which is the size of the
 // rounding of the result; their sum is taken of the f32 values.
 //
+// CS > 1: the columns of v and of the result are divided over CS workgroups, each of which forms all the scores.  At D = 256 that halves
+// the registers of o: two workgroups of a CU instead of one hide each other's latencies in bf16, 4 x 1000 x 2000 keys of 4 heads 70 us
+// against 83, 8 x 1444 x 2704 of 8 heads 420 against 460.  f32 takes it where the tiles do not fill the GPU (4 x 559 x 30 keys of 2 heads 16.8 us
+// against 23.2), not elsewhere (8 x 1444 x 1444 of 4 heads 1093 against 906: its products bound it).
+//
 // LDS rows are the next power of two of the head size.  k: 16-byte piece c of a row at c ^ f(row) so that 16 rows' pieces fall on
 // all banks; v: 64-byte (f32: 128-byte) blocks exchanged likewise for the transposed reads of four rows at a time.
 __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
@@ -133,7 +138,6 @@ template <bool BF16, int DC> struct AttnTile {
     static constexpr int PCS = ROW / 16, KT = ROW >= 512 ? 32 : 64;                  // pieces of an LDS row, keys per tile
     static constexpr int RPL = ROW >= 256 ? 1 : 256 / ROW;                          // rows per 256 bytes (all banks)
     static constexpr int TILE = KT * ROW;                                           // bytes of one k or v tile
-    static constexpr int LDS = 4 * TILE;
     static constexpr int BLK = BF16 ? 4 : 8;                                        // pieces of a v block
     static __device__ __forceinline__ int kpiece(int row, int c) { return c ^ ((row / RPL) & (PCS - 1)); }
     static __device__ __forceinline__ int vpiece(int row, int c) {
@@ -144,21 +148,24 @@ template <bool BF16, int DC> struct AttnTile {
     }
 };
 
-template <bool BF16, int DC, int WAVES, int MW>
+template <bool BF16, int DC, int WAVES, int MW, int CS>
 __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(AttnK p) {
     typedef typename Elem<BF16>::type T;
-    typedef AttnTile<BF16, DC> L;
+    typedef AttnTile<BF16, DC> L;                           // k
+    typedef AttnTile<BF16, DC / CS> LV;                     // v: DC / CS columns of as many keys
     constexpr int P = L::P, PCS = L::PCS, KT = L::KT, NT = WAVES * 64;
     constexpr int QS = DC / (2 * P);                        // k steps of S: two pieces (one per lane half) each
-    constexpr int DT = DC / 32, KB = KT / 32;               // 32-wide tiles of o, 32-key tiles of S
+    constexpr int DT = DC / CS / 32, KB = KT / 32;          // 32-wide tiles of o, 32-key tiles of S
     constexpr int RPI = NT / PCS;                           // rows a pass of all threads stages
-    constexpr int NI = KT / RPI;
-    static_assert(KT % RPI == 0, "whole passes");
+    constexpr int NI = KT / RPI, VRPI = NT / LV::PCS, VNI = KT / VRPI, VTILE = KT * LV::ROW;
+    static_assert(KT % RPI == 0 && KT % VRPI == 0, "whole passes");
     extern __shared__ char lds[];                           // k0 k1 v0 v1
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
     unsigned id = xcd_chunk(blockIdx.x, gridDim.x);
+    const int c0 = (int)(id % CS) * (DC / CS);              // first column of v and of the result
+    id /= CS;
     const int rt = (int)(id % p.rtiles);
     id /= p.rtiles;
     const int split = (int)(id % p.splits);
@@ -194,11 +201,11 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[i][r] = 0.f;
 
-    // staging: thread covers slot tid % PCS of rows tid / PCS + RPI i
-    const int r0 = tid / PCS, slot = tid % PCS;
+    // staging: thread covers slot tid % PCS of rows tid / PCS + RPI i; of v likewise
+    const int r0 = tid / PCS, slot = tid % PCS, vr0 = tid / LV::PCS, vslot = tid % LV::PCS;
     const long long kls = p.kl * (long long)sizeof(T), vls = p.vl * (long long)sizeof(T);
     const char* kbase = p.k + (b * p.kb + hk * p.kh) * (long long)sizeof(T);
-    const char* vbase = p.v + (b * p.vb + hk * p.vh) * (long long)sizeof(T);
+    const char* vbase = p.v + (b * p.vb + hk * p.vh + c0) * (long long)sizeof(T);
     const uint8_t* mrow = p.mask ? p.mask + (long long)b * p.Lk : nullptr;
     auto mask_byte = [&](int t) {                           // lane = key of tile t; 0 beyond the last key
         const int j = t * KT + lane;
@@ -213,23 +220,23 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
     const bool padded = p.D * L::Z != L::ROW;
     auto issue = [&](int t, int buf, unsigned long long kept) {
         char* kd = lds + buf * L::TILE + wave * 1024;
-        char* vd = lds + (2 + buf) * L::TILE + wave * 1024;
+        char* vd = lds + 2 * L::TILE + buf * VTILE + wave * 1024;
         const char* ks = kbase + ((long long)t * KT + r0) * kls;
-        const char* vs = vbase + ((long long)t * KT + r0) * vls;
+        const char* vs = vbase + ((long long)t * KT + vr0) * vls;
         auto each_piece = [&](auto plain) {
 #pragma unroll
             for (int i = 0; i < NI; ++i) {
-                const int r = r0 + i * RPI;
-                const int kc = L::kpiece(r, slot), vc = L::vpiece(r, slot);
-                const char* kg = ks + (long long)(i * RPI) * kls + kc * 16;
-                const char* vg = vs + (long long)(i * RPI) * vls + vc * 16;
-                if constexpr (!plain.value) {
-                    const bool in = (kept >> r) & 1;
-                    kg = in && kc * P < p.D ? kg : (const char*)&kZeroPiece;
-                    vg = in && vc * P < p.D ? vg : (const char*)&kZeroPiece;
-                }
-                dma16(kg, kd + i * NT * 16);
-                dma16(vg, vd + i * NT * 16);
+                const int r = r0 + i * RPI, c = L::kpiece(r, slot);
+                const char* g = ks + (long long)(i * RPI) * kls + c * 16;
+                if constexpr (!plain.value) g = ((kept >> r) & 1) && c * P < p.D ? g : (const char*)&kZeroPiece;
+                dma16(g, kd + i * NT * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < VNI; ++i) {
+                const int r = vr0 + i * VRPI, c = LV::vpiece(r, vslot);
+                const char* g = vs + (long long)(i * VRPI) * vls + c * 16;
+                if constexpr (!plain.value) g = ((kept >> r) & 1) && c0 + c * P < p.D ? g : (const char*)&kZeroPiece;
+                dma16(g, vd + i * NT * 16);
             }
         };
         if (!padded && (kept & full) == full) each_piece(std::true_type{});
@@ -254,7 +261,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
             mb = mask_byte(t + 2);
         }
         const char* kt = lds + buf * L::TILE;
-        const char* vt = lds + (2 + buf) * L::TILE;
+        const char* vt = lds + 2 * L::TILE + buf * VTILE;
 
         f32x16 s[KB];
 #pragma unroll
@@ -342,9 +349,9 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
                         const int e = i * 32 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;             // first element
                         const int c = e / 8, w = (e & 7) * 2;
                         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                            (__attribute__((address_space(3))) char*)vt + key * L::ROW + L::vpiece(key, c) * 16 + w));
+                            (__attribute__((address_space(3))) char*)vt + key * LV::ROW + LV::vpiece(key, c) * 16 + w));
                         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                            (__attribute__((address_space(3))) char*)vt + (key + 8) * L::ROW + L::vpiece(key + 8, c) * 16 + w));
+                            (__attribute__((address_space(3))) char*)vt + (key + 8) * LV::ROW + LV::vpiece(key + 8, c) * 16 + w));
                         typedef short s16x8 __attribute__((ext_vector_type(8)));
                         const bf16x8 fv = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv, fp, o[i], 0, 0, 0);
@@ -357,7 +364,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
 #pragma unroll
                     for (int i = 0; i < DT; ++i) {
                         const int e = i * 32 + col;
-                        const float fv = *(const float*)(vt + key * L::ROW + L::vpiece(key, e / 4) * 16 + (e & 3) * 4);
+                        const float fv = *(const float*)(vt + key * LV::ROW + LV::vpiece(key, e / 4) * 16 + (e & 3) * 4);
                         o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(fv, s[kb][r], o[i], 0, 0, 0);
                     }
                 }
@@ -370,7 +377,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
     const bool in = row < rows;
     const bool parts = p.part != nullptr;
     const float f = parts ? 1.0f : any ? 1.0f / l : 0.f;
-    if (in && parts && half == 0) p.ml[split * total + orow] = make_float2(mref, any ? l : -1.0f);
+    if (in && parts && half == 0 && c0 == 0) p.ml[split * total + orow] = make_float2(mref, any ? l : -1.0f);
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
 #pragma unroll
@@ -385,7 +392,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
                 v[j] = __uint_as_float(sw[0]);
                 v[4 + j] = __uint_as_float(sw[1]);
             }
-            const int d = i * 32 + 16 * g + 8 * half;
+            const int d = c0 + i * 32 + 16 * g + 8 * half;
             if (!in || d >= p.D) continue;              // D is whole groups of 8
             if (parts || !BF16) {
                 float* dst = parts ? p.part + (split * total + orow) * p.D + d : (float*)p.out + orow * p.D + d;
@@ -498,7 +505,7 @@ __global__ __launch_bounds__(256) void cross_attention_join_rows_kernel(AttnK p)
 
 // ---- plan: the tile shape and the number of key splits, by sizes and type alone ---------------------------------------------------
 struct AttnPlan {
-    int dc, waves, kt, rtiles, splits, tps;
+    int dc, waves, kt, rtiles, cs, splits, tps;     // cs: column parts of v
     size_t bytes;
 };
 
@@ -520,12 +527,12 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     const int tiles = (Lk + a.kt - 1) / a.kt;
     if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) a.waves = 8;
     a.rtiles = (int)rtiles(a.waves);
-    const long long blocks = a.rtiles * groups;
+    const long long blocks = a.rtiles * groups;             // times the column parts
     // a round: 256 workgroups, one to a CU, take `one` us a tile (latency), 512 of four waves `two` (one where a wave has the whole
     // register file); one-wave workgroups run as many to a CU as their LDS allows
     const int row_bytes = a.dc <= 32 ? (bf16 ? 64 : 128) : a.dc <= 64 ? (bf16 ? 128 : 256) : a.dc <= 128 ? (bf16 ? 256 : 512) : (bf16 ? 512 : 1024);
     const double part = a.dc / 64.0 * a.kt / 64.0;
-    const bool pairs = a.waves == 4 && a.dc < 256 && (bf16 || a.dc <= 64);
+    const bool pairs = a.waves == 4 && (bf16 || a.dc <= 64);
     const double one = a.waves == 1 ? (bf16 ? 0.3 + 0.8 * part : 5.0 * part) : a.waves == 8 ? 0.6 + 0.75 * part : bf16 ? 0.5 + 0.45 * part : 4.8 * part;
     const double two = bf16 ? 0.6 + 0.8 * part : 7.5 * part;
     const long long per_cu = a.waves != 1 ? 1 : 160 * 1024 / (4 * a.kt * row_bytes) < 4 ? 160 * 1024 / (4 * a.kt * row_bytes) : 4;
@@ -536,15 +543,18 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     const double join_fixed_us = a.waves == 1 ? 7.0 : 4.0;                          // where latency counts also the launch on the host
     const double join_us = 4e-6 * 2 * B * Lq * (double)Hq * D / 4;                  // of one more split, at 4 TB/s
     double best = 0;
-    a.splits = 1;
-    a.tps = tiles;
-    for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
-        const int tps = (tiles + s - 1) / s, splits = (tiles + tps - 1) / tps;
-        const double t = tile_us(blocks * splits) * (tps + 1.5) + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
-        if (s == 1 || t < best) {
-            best = t;
-            a.splits = splits;
-            a.tps = tps;
+    a.cs = 0;
+    for (int cs = bf16 && a.dc == 256 ? 2 : 1; cs <= (a.dc == 256 ? 2 : 1); ++cs) {
+        const double share = !bf16 && cs == 2 ? 2.0 / 3 : 1.0;                      // f32: scores and half of the results
+        for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
+            const int tps = (tiles + s - 1) / s, splits = (tiles + tps - 1) / tps;
+            const double t = tile_us(blocks * cs * splits) * share * (tps + 1.5) + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
+            if (a.cs == 0 || t < best) {
+                best = t;
+                a.cs = cs;
+                a.splits = splits;
+                a.tps = tps;
+            }
         }
     }
     a.bytes = a.splits > 1 ? (size_t)a.splits * B * Lq * Hq * (D + 2) * 4 : 0;
@@ -552,23 +562,23 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
 }
 
 // MW: waves per SIMD the register budget is cut for.  Two hide each other's latencies where the tiles fill the GPU (D = 128, four waves:
-// 804 us at one, 553 at two); one-wave workgroups run one to a SIMD, and 256 elements of o, q and their tiles need all 512 registers
-template <bool BF16, int DC, int WAVES, int MW = (WAVES == 1 || DC == 256 || (!BF16 && DC > 64)) ? 1 : 2>
+// 804 us at one, 553 at two); one-wave workgroups run one to a SIMD, and f32 with more than 64 elements of o and q needs all 512 registers
+template <bool BF16, int DC, int WAVES, int CS = 1, int MW = (WAVES == 1 || (!BF16 && DC > 64)) ? 1 : 2>
 static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
-    constexpr int kLds = AttnTile<BF16, DC>::LDS;
+    constexpr int kLds = 2 * AttnTile<BF16, DC>::TILE + 2 * AttnTile<BF16, DC>::KT * AttnTile<BF16, DC / CS>::ROW;
     if (kLds > 64 * 1024) {
         static std::atomic<bool> attr_done[16];   // setting the attribute twice is harmless, the flag only must not tear
         int dev = 0;
         YOLO_HIP_CHECK(hipGetDevice(&dev));
         if (dev >= 16 || !attr_done[dev]) {
-            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, MW>,
+            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS>,
                                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
             if (dev < 16) attr_done[dev] = true;
         }
     }
-    const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk;
+    const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk * CS;
     YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 workgroups");
-    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, MW>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
+    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
@@ -581,7 +591,10 @@ static int launch_attn_dc(const AttnK& p, const AttnPlan& a, hipStream_t stream)
     if constexpr (DC < 256) {
         if (a.waves == 1) return launch_attn_tile<BF16, DC, 1>(p, stream);
     }
-    return launch_attn_tile<BF16, DC, 4>(p, stream);
+    if constexpr (DC == 256) {
+        if (BF16 || a.cs == 2) return launch_attn_tile<BF16, DC, 4, 2>(p, stream);
+    }
+    if constexpr (!BF16 || DC < 256) return launch_attn_tile<BF16, DC, 4>(p, stream);
 }
 
 template <bool BF16>
