@@ -378,6 +378,19 @@ def test_attention_wide_heads(L, t, d, b, lq, lk, hq, hk):
 
 
 @pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 160, 256])
+@pytest.mark.parametrize("lq,lk", [(55, 73), (20, 96), (300, 130)])
+def test_attention_several_workgroups_on_a_cu(L, t, d, lq, lk):
+    """More workgroups than CUs and more than one tile of keys: neighbours that share a CU do not disturb each other."""
+    q, k, v = qkv(t, 30, lq, lk, 16, 4, d, 72)
+    lens = torch.randint(lk // 2, lk + 1, (30,), generator=torch.Generator().manual_seed(6), dtype=torch.int32).cuda()
+    full = check_attention(L, q, k, v, what=(t, d, lq, lk))
+    for _ in range(3):
+        assert torch.equal(L.cross_attention(q, k, v), full)
+    check_attention(L, q, k, v, lens=lens, what=("lens", t, d, lq, lk))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
 def test_attention_scales_and_extreme_scores(L, t):
     q, k, v = qkv(t, 2, 50, 333, 4, 4, 64, 60)
     for scale in (0.0, -0.2, 1.0, 3.0):

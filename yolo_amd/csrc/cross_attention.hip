@@ -211,10 +211,21 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
         const int j = t * KT + lane;
         return (mrow && lane < KT && j < n) ? (int)mrow[j] : 0;
     };
+    // The mask of a tile is the wave's, in scalar registers, and is read in 32-bit words: a 64-bit shift by a vector count gave wrong masks
+    // where the count sat in the last of 256 registers and two such waves filled a SIMD's register file.
     auto kept_bits = [&](int t, int mb) -> unsigned long long {
-        if (mrow) return __ballot(mb != 0);
-        const int left = n - t * KT;
-        return left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1ull;
+        unsigned long long bits;
+        if (mrow) {
+            bits = __ballot(mb != 0);
+        } else {
+            const int left = __builtin_amdgcn_readfirstlane(n - t * KT);
+            bits = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1ull;
+        }
+        return (unsigned long long)(uint32_t)__builtin_amdgcn_readfirstlane((int)(bits >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)bits);
+    };
+    auto kept_row = [](unsigned long long bits, int r) {
+        const uint32_t word = KT == 64 && r >= 32 ? (uint32_t)(bits >> 32) : (uint32_t)bits;
+        return ((word >> (r & 31)) & 1u) != 0;
     };
     const unsigned long long full = KT == 64 ? ~0ull : 0xffffffffull;
     const bool padded = p.D * L::Z != L::ROW;
@@ -228,14 +239,14 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
             for (int i = 0; i < NI; ++i) {
                 const int r = r0 + i * RPI, c = L::kpiece(r, slot);
                 const char* g = ks + (long long)(i * RPI) * kls + c * 16;
-                if constexpr (!plain.value) g = ((kept >> r) & 1) && c * P < p.D ? g : (const char*)&kZeroPiece;
+                if constexpr (!plain.value) g = kept_row(kept, r) && c * P < p.D ? g : (const char*)&kZeroPiece;
                 dma16(g, kd + i * NT * 16);
             }
 #pragma unroll
             for (int i = 0; i < VNI; ++i) {
                 const int r = vr0 + i * VRPI, c = LV::vpiece(r, vslot);
                 const char* g = vs + (long long)(i * VRPI) * vls + c * 16;
-                if constexpr (!plain.value) g = ((kept >> r) & 1) && c0 + c * P < p.D ? g : (const char*)&kZeroPiece;
+                if constexpr (!plain.value) g = kept_row(kept, r) && c0 + c * P < p.D ? g : (const char*)&kZeroPiece;
                 dma16(g, vd + i * NT * 16);
             }
         };
@@ -283,12 +294,11 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
         }
         if ((kept & full) != full) {
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int kb = 0; kb < KB; ++kb) {
+                const uint32_t lane_keys = (uint32_t)(kept >> (32 * kb)) >> (4 * half);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool in = (kept >> (kb * 32 + 8 * (r >> 2) + 4 * half + (r & 3))) & 1;
-                    s[kb][r] = in ? s[kb][r] : -__builtin_inff();
-                }
+                for (int r = 0; r < 16; ++r) s[kb][r] = lane_keys & (1u << (8 * (r >> 2) + (r & 3))) ? s[kb][r] : -__builtin_inff();
+            }
         }
         any |= kept != 0;
         kept = next;

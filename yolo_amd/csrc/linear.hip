@@ -111,7 +111,11 @@ __device__ __forceinline__ u32x4 place_piece(u32x4 v, int k, int K) {
     const int excess = k + P - K;
     if (excess <= 0) return v;
     if (excess >= P) return u32x4{0, 0, 0, 0};
-    return __builtin_bit_cast(u32x4, __builtin_bit_cast(unsigned __int128, v) >> (excess * Z * 8));
+    const int bytes = excess * Z;                           // in 32-bit steps: see the masks of cross_attention_tile_kernel
+    if (bytes & 8) v = u32x4{v[2], v[3], 0, 0};
+    if (bytes & 4) v = u32x4{v[1], v[2], v[3], 0};
+    if (bytes & 2) v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+    return v;
 }
 
 // ---- tiles of BM rows of x by BN rows of W through LDS ------------------------------------------------------------------------
