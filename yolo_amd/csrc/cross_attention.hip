@@ -5,6 +5,7 @@
 // o <- o exp(m - m') + sum exp(s - m') v and l likewise, result o / l.  Scores, m, l and o are f32.  A key is kept when its
 // index is below key_lens[b] and its key_mask byte is set; what is not kept is never multiplied (its score is replaced, its
 // value row not used), so that infinities and NaN there stay out.  A row without a kept key is zero.
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -525,6 +526,9 @@ struct AttnPlan {
 // heads of 64, 4 key heads: 9.1 at S = 1, 8.5 at 5 over 300 keys; 28 at 1, 8.9 at 12 over 1444; 64 at 1, 10 at 28 over 3549.
 // Eight waves share a tile's loads where their larger row tiles still fill the CUs as well (8 x 2704 queries of 8 heads of 128: 524
 // against 553), not over few tiles (80 keys, above: 153).
+// Up to 32 rows of a head group need one wave, but four load a tile faster while CUs are free (one query of 16 / 4 heads of 64 over 3549 keys
+// 9.4 against 10.3 us, 2 of 2 heads of 96 over 217: 8.4 against 13.2), and at 96 and more in bf16 as many workgroups of four waves fit a CU as of one;
+// one-wave workgroups where they fill the CUs several times (16 x that query 19 against 23, f32 54 against 72).
 static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
     AttnPlan a;
     const bool bf16 = dtype == YOLO_DTYPE_BF16;
@@ -533,39 +537,50 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     const long long rows = (long long)Lq * (Hq / Hk), groups = (long long)B * Hk;
     auto rtiles = [&](int waves) { return (rows + 32 * waves - 1) / (32 * waves); };
     auto rounds = [](long long blocks, long long slots) { return (blocks + slots - 1) / slots; };
-    a.waves = rows <= 32 && a.dc < 256 ? 1 : 4;
+    const bool few = rows <= 32;
     const int tiles = (Lk + a.kt - 1) / a.kt;
-    if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) a.waves = 8;
-    a.rtiles = (int)rtiles(a.waves);
-    const long long blocks = a.rtiles * groups;             // times the column parts
-    // a round: 256 workgroups, one to a CU, take `one` us a tile (latency), 512 of four waves `two` (one where a wave has the whole
-    // register file); one-wave workgroups run as many to a CU as their LDS allows
+    int wide = 4;                                           // waves of a workgroup where there are rows for more than one
+    if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) wide = 8;
+    // one tile of n workgroups, us: where each has a CU `one`; two workgroups of four waves share a CU in `two`, one-wave workgroups as many
+    // as their LDS allows, a quarter longer for each more (f32 above 64 elements: one to a CU)
     const int row_bytes = a.dc <= 32 ? (bf16 ? 64 : 128) : a.dc <= 64 ? (bf16 ? 128 : 256) : a.dc <= 128 ? (bf16 ? 256 : 512) : (bf16 ? 512 : 1024);
     const double part = a.dc / 64.0 * a.kt / 64.0;
-    const bool pairs = a.waves == 4 && (bf16 || a.dc <= 64);
-    const double one = a.waves == 1 ? (bf16 ? 0.3 + 0.8 * part : 5.0 * part) : a.waves == 8 ? 0.6 + 0.75 * part : bf16 ? 0.5 + 0.45 * part : 4.8 * part;
-    const double two = bf16 ? 0.6 + 0.8 * part : 7.5 * part;
-    const long long per_cu = a.waves != 1 ? 1 : 160 * 1024 / (4 * a.kt * row_bytes) < 4 ? 160 * 1024 / (4 * a.kt * row_bytes) : 4;
-    auto tile_us = [&](long long n) {                                               // n workgroups, one tile each
-        if (!pairs) return rounds(n, 256 * per_cu) * one;
+    const int per_cu = std::min(4, 160 * 1024 / (4 * a.kt * row_bytes));
+    auto tile_us = [&](int waves, long long n) {
+        if (waves == 1) {
+            const double one = bf16 ? 0.8 + 0.6 * part : 5.0 * part;
+            return rounds(n, 256 * per_cu) * one * (0.75 + 0.25 * std::min<long long>(per_cu, rounds(n, 256)));
+        }
+        const double one = waves == 8 ? 0.6 + 0.75 * part : bf16 ? 0.5 + 0.45 * part : 4.8 * part;
+        if (waves == 8 || (!bf16 && a.dc > 64)) return rounds(n, 256) * one;
+        const double two = bf16 ? (few ? 0.7 + 0.95 * part : 0.6 + 0.8 * part) : 7.5 * part;
         return n / 512 * two + (n % 512 == 0 ? 0.0 : n % 512 <= 256 ? one : two);
     };
-    const double join_fixed_us = a.waves == 1 ? 7.0 : 4.0;                          // where latency counts also the launch on the host
+    const double join_fixed_us = few ? 7.0 : 4.0;                                   // where latency counts also the launch on the host
     const double join_us = 4e-6 * 2 * B * Lq * (double)Hq * D / 4;                  // of one more split, at 4 TB/s
     double best = 0;
-    a.cs = 0;
-    for (int cs = bf16 && a.dc == 256 ? 2 : 1; cs <= (a.dc == 256 ? 2 : 1); ++cs) {
-        const double share = !bf16 && cs == 2 ? 2.0 / 3 : 1.0;                      // f32: scores and half of the results
+    a.splits = 0;
+    auto consider = [&](int waves, int cs, double share) {
+        const int rt = (int)rtiles(waves);
         for (int s = 1; s <= kMaxSplits && s <= tiles; ++s) {
             const int tps = (tiles + s - 1) / s, splits = (tiles + tps - 1) / tps;
-            const double t = tile_us(blocks * cs * splits) * share * (tps + 1.5) + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
-            if (a.cs == 0 || t < best) {
+            const double t = tile_us(waves, rt * groups * cs * splits) * share * (tps + 1.5) + (splits > 1 ? join_fixed_us + splits * (0.04 + join_us) : 0.0);
+            if (a.splits == 0 || t < best) {
                 best = t;
+                a.waves = waves;
+                a.rtiles = rt;
                 a.cs = cs;
                 a.splits = splits;
                 a.tps = tps;
             }
         }
+    };
+    if (a.dc == 256) {
+        if (!bf16) consider(4, 1, 1.0);
+        consider(4, 2, bf16 ? 1.0 : 2.0 / 3);               // f32: scores and half of the results
+    } else {
+        consider(wide, 1, 1.0);
+        if (few && (!bf16 || a.dc <= 64)) consider(1, 1, 1.0);
     }
     a.bytes = a.splits > 1 ? (size_t)a.splits * B * Lq * Hq * (D + 2) * 4 : 0;
     return a;
@@ -598,7 +613,7 @@ static int launch_attn_dc(const AttnK& p, const AttnPlan& a, hipStream_t stream)
     if constexpr (BF16 && (DC == 64 || DC == 96 || DC == 128)) {
         if (a.waves == 8) return launch_attn_tile<BF16, DC, 8>(p, stream);
     }
-    if constexpr (DC < 256) {
+    if constexpr (DC <= 64 || (!BF16 && DC < 256)) {
         if (a.waves == 1) return launch_attn_tile<BF16, DC, 1>(p, stream);
     }
     if constexpr (DC == 256) {
