@@ -762,3 +762,21 @@ def test_attention_odd_head_sizes_through_the_c_entry(L, t, d):
         cross_attention = staticmethod(call)
     check_attention(Entry, q, k, v, lens, mask, what=("c entry", d))
     check_attention(L, q, k, v, lens, mask, what=("padded", d))
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("n", [16, 640])                       # the direct kernel and a tile kernel
+def test_gelu_is_relatively_exact_in_the_negative_tail(L, t, n):
+    """Every bfloat16 from -2^-10 to -12.75 as an exact pre-activation: the result is within its rounding and 2^-13 of y itself (bfloat16: the
+    formula is within 2^-14; float32: the error function's sixteen last places at most), and v^2 2^-22 of y for the rounded argument
+    of the exponential: v^2 / 2 times four roundings of 2^-24."""
+    v = -(torch.arange(int(12.75 * 2 ** 7), 0, -1).double() * 2.0 ** -7)            # to -2^-7 ..
+    v = torch.cat([v, -(torch.arange(128, 256).double()[:, None] * 2.0 ** -torch.arange(7, 18).double()).flatten()]).to(BF16).to(t).cuda()      # .. octaves to -2^-10
+    x, w = torch.zeros((v.numel(), 8), dtype=t, device="cuda"), torch.zeros((n, 8), dtype=t, device="cuda")
+    x[:, 0], w[:, 0] = v, 1
+    v64 = v.double().cpu()
+    y = v64 * 0.5 * torch.special.erfc(-v64 * 0.5 ** 0.5)      # torch's ndtr is 1 + erf, which leaves nothing of the tail below -8.3
+    u, formula = torch.finfo(t).eps / 2, 2.0 ** -13 if t == BF16 else 2.0 ** -19
+    bound = (u * (1 + formula) + formula + v64 * v64 * 2.0 ** -22) * y.abs() + 1e-38
+    got = L.linear(x, w, activation="gelu")
+    within(got, y[:, None].expand(-1, n), bound[:, None].expand(-1, n), (t, n))
