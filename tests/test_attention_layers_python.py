@@ -1,0 +1,51 @@
+"""CPU: what the Python functions of the attention-side layers refuse or resolve before they call the library.  CPU tensors pass as those
+of the current GPU, and the library is one that no call may reach."""
+import pytest
+import torch
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+class Unreachable:
+    def __getattr__(self, name):
+        raise AssertionError("%s was called" % name)
+
+
+@pytest.fixture
+def L(monkeypatch):
+    from yolo_amd import _lib
+    from yolo_amd.utils import layer_utils
+    monkeypatch.setattr(layer_utils, "_gpu", lambda: -1)                            # get_device() of a CPU tensor
+    monkeypatch.setattr(_lib, "lib", Unreachable)
+    layer_utils._attention_workspace.cache_clear()
+    yield layer_utils
+    layer_utils._attention_workspace.cache_clear()
+
+
+def refused(call, text):
+    with pytest.raises(ValueError, match=text):
+        call()
+
+
+def huge(*shape):
+    """A tensor of more than 2^31 along one dimension; its pages are never touched."""
+    return torch.empty(shape, dtype=BF16)
+
+
+def test_sizes_past_32_bits_are_refused(L):
+    """The C entries take int sizes, and ctypes passes the low 32 bits of a longer one: 2^32 + 8 would run as 8."""
+    n = 2 ** 32 + 8
+    refused(lambda: L.linear(huge(1, n), huge(1, n)), "2\\^31")
+    refused(lambda: L.linear(huge(2, 1), huge(n, 1)), "2\\^31")
+    one = huge(1, 1, 1, 8)
+    refused(lambda: L.cross_attention(one, huge(1, n, 1, 1).expand(1, n, 1, 8), huge(1, n, 1, 1).expand(1, n, 1, 8)), "2\\^31")
+    refused(lambda: L.cross_attention(huge(1, n, 1, 1), huge(1, 1, 1, 1), huge(1, 1, 1, 1)), "2\\^31")
+    refused(lambda: L.cross_attention(huge(1, 1, n, 1), huge(1, 1, 1, 1), huge(1, 1, 1, 1)), "2\\^31")
+    refused(lambda: L.cross_attention(huge(n, 1, 1, 1), huge(n, 1, 1, 1), huge(n, 1, 1, 1)), "2\\^31")
+    refused(lambda: L.cross_attention(huge(1, 1, 1, n), huge(1, 1, 1, n), huge(1, 1, 1, n)), "2\\^31")
+    refused(lambda: L.qk_norm_rope(huge(n, 1, 1, 1), None), "2\\^31")
+    refused(lambda: L.qk_norm_rope(huge(1, n, 1, 1), None), "2\\^31")
+    refused(lambda: L.qk_norm_rope(huge(1, 1, n, 1), None), "2\\^31")
+    refused(lambda: L.qk_norm_rope(huge(1, 1, 1, n), None), "2\\^31")
+    refused(lambda: L.qk_norm_rope(one, huge(1, n, 1, 1).expand(1, n, 1, 8)), "2\\^31")
+    refused(lambda: L.qk_norm_rope(one, huge(1, 1, n, 1).expand(1, 1, n, 8)), "2\\^31")

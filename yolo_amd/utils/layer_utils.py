@@ -190,6 +190,12 @@ def _param(x, n, name, dev):
     return x.contiguous(), _code(x, name)
 
 
+def _fits(name, *sizes):
+    """The C entries take int sizes, and ctypes would pass on the low 32 bits of a longer one."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError("%s: sizes %s, each must be below 2^31" % (name, sizes))
+
+
 def _gpu():
     """Index of the current GPU; like `_tensor.device()` an error without one."""
     try:
@@ -236,6 +242,7 @@ def linear(inputs, weight, bias=None, activation=None, residual=None):
     if not shape or len(wshape) != 2 or wshape[1] != shape[-1] or wshape[1] == 0 or wshape[0] == 0:
         raise ValueError("linear: inputs %s do not fit weight %s" % (shape, tuple(wshape)))
     N, K = wshape
+    _fits("linear", N, K)
     b, bcode = _param(bias, N, "bias", dev)
     shape = shape[:-1] + (N,)
     r, r_ld = None, 0
@@ -266,6 +273,7 @@ def _heads(x, name):
     """[B, L, H, D] with a contiguous last dimension -> (tensor, ctypes strides of batch, token, head)."""
     if x.dim() != 4:
         raise ValueError("%s must be [B, L, H, D], got %s" % (name, tuple(x.shape)))
+    _fits(name, *x.shape)
     st = x.stride()
     if st[3] != 1 and x.shape[3] > 1:
         x = x.contiguous()
@@ -373,6 +381,7 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
         raise ValueError("cross_attention: q %s and k %s must be [B, L, H, D]" % (tuple(q.shape), tuple(k.shape)))
     B, Lq, Hq, D = q.shape
     Lk, Hk = k.shape[1:3]
+    _fits("cross_attention", B, Lq, Lk, Hq, Hk, D)
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
         raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
