@@ -49,3 +49,14 @@ def test_sizes_past_32_bits_are_refused(L):
     refused(lambda: L.qk_norm_rope(huge(1, 1, 1, n), None), "2\\^31")
     refused(lambda: L.qk_norm_rope(one, huge(1, n, 1, 1).expand(1, n, 1, 8)), "2\\^31")
     refused(lambda: L.qk_norm_rope(one, huge(1, 1, n, 1).expand(1, 1, n, 8)), "2\\^31")
+
+
+def test_lazily_negated_tensors_hold_their_values(L):
+    """The imaginary part of a conjugate is a view with torch's negative bit: its memory holds the values' negatives."""
+    z = torch.complex(torch.arange(8.0), torch.arange(8.0) + 1)
+    x = torch.conj(z).imag
+    assert x.is_neg()
+    got = L._dev(x, "x", -1)
+    assert not got.is_neg() and torch.equal(got, -(torch.arange(8.0) + 1))
+    same = torch.arange(8.0)
+    assert L._dev(same, "x", -1) is same

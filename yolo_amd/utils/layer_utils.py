@@ -160,6 +160,8 @@ def _dev(x, name, dev, dtype=None):
             x = x.float()
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires a gradient: yolo_amd implements the inference path only (call under torch.no_grad())" % name)
+    if x.is_neg():                                                    # imaginary part of a conjugate: memory holds the negatives
+        x = x.resolve_neg()
     if dtype is not None and x.dtype != dtype:
         x = x.to(dtype)
     if x.get_device() != dev:
