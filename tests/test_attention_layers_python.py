@@ -60,3 +60,31 @@ def test_lazily_negated_tensors_hold_their_values(L):
     assert not got.is_neg() and torch.equal(got, -(torch.arange(8.0) + 1))
     same = torch.arange(8.0)
     assert L._dev(same, "x", -1) is same
+
+
+def test_forward_mode_derivatives_are_refused(L):
+    """A dual tensor of torch.autograd.forward_ad would come out without its tangent.  Like requires_grad it is refused, for every operand;
+    plain tensors inside a dual level are not."""
+    from torch.autograd import forward_ad
+    x, w, b = torch.randn(3, 8), torch.randn(4, 8), torch.randn(4)
+    q, k = torch.randn(1, 2, 2, 8), torch.randn(1, 3, 1, 8)
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+        for i in range(4):
+            a = [x, w, b, torch.randn(3, 4)]
+            a[i] = dual(a[i])
+            refused(lambda: L.linear(a[0], a[1], a[2], residual=a[3]), "tangent")
+            with torch.no_grad():
+                refused(lambda: L.linear(a[0], a[1], a[2], residual=a[3]), "tangent")
+        for i in range(3):
+            a = [q, k, k.clone()]
+            a[i] = dual(a[i])
+            refused(lambda: L.cross_attention(*a), "tangent")
+        n = torch.ones(8)
+        for i in range(4):
+            a = [q, k, n, n.clone()]
+            a[i] = dual(a[i])
+            refused(lambda: L.qk_norm_rope(*a), "tangent")
+        with pytest.raises(AssertionError, match="yolo_linear was called"):
+            L.linear(x, w, b)
