@@ -236,7 +236,8 @@ int yolo2_nms(const double* boxes, const float* probs, int B, int n, int C, floa
  * rounds the weights of the values).  Outputs must not overlap inputs; memory the outputs do not name is left as it was.  None
  * allocates, synchronises or keeps anything between calls, so calls may overlap on any streams (each with a workspace of its
  * own) and may be captured into a HIP graph.  A call repeated gives the same bits; the kernel and the order of its sums go by the
- * sizes of the call, so a row may differ in its last bits between calls of other batch sizes. */
+ * sizes of the call, so a row may differ in its last bits between calls of other batch sizes.  Sizes that need 2^32 threads or more in a
+ * launch (2^24 workgroups of 256) are YOLO_ERR_UNSUPPORTED. */
 enum { YOLO_ACT_NONE = 0, YOLO_ACT_LEAKY = 1, YOLO_ACT_RELU = 2, YOLO_ACT_GELU = 3, YOLO_ACT_SILU = 4 };
 
 /* out[m,n] = act(sum_k x[m,k] * weight[n,k] + bias[n]) + residual[m,n]: the 1x1 conv2d of a feature map's cells (yolo_conv_forward)

@@ -73,3 +73,16 @@ def test_cross_attention(L):
         a = dict(dtype=1, B=1, Lq=1, Lk=100, Hq=4, Hk=2, D=64)
         a.update(bad)
         assert L.yolo_cross_attention_workspace_bytes(*a.values()) == 0
+
+
+def test_launches_past_the_runtime_limit_are_refused(L):
+    """The runtime counts the threads of a launch in 32 bits: sizes that need more are the documented refusal, not a failed launch."""
+    for kw in (dict(M=1 << 30, N=1, out_ld=1), dict(M=1 << 30, N=256, out_ld=256), dict(M=1 << 30, N=256, out_ld=256, dtype=0),
+               dict(M=1 << 30, N=256, out_ld=256, x_ld=9), dict(M=1 << 30, N=33, out_ld=33, x_ld=1 << 22)):
+        assert linear(L, **kw) == UNSUPPORTED and b"tiles" in L.yolo_last_error(), (kw, L.yolo_last_error())
+    wide = dict(qs=strides(1 << 20, 256, 8), D=8, R=8)
+    for kw in (dict(wide, B=1 << 12, Lq=1 << 12, Hq=32), dict(B=1 << 12, Lq=1 << 12, Hq=64, D=256, R=256), dict(wide, B=1 << 12, Lq=1 << 12, Hq=32, D=4, R=4, dtype=0)):
+        assert qk(L, **kw) == UNSUPPORTED and b"workgroups" in L.yolo_last_error(), (kw, L.yolo_last_error())
+    for kw in (dict(B=1 << 10, Lq=1 << 13, Hq=8, Hk=8, Lk=0), dict(B=1 << 10, Lq=1 << 13, Hq=8, Hk=8, D=7), dict(B=1 << 26, Hq=1, Hk=1),
+               dict(B=1 << 24, Hq=1, Hk=1, D=128), dict(B=1 << 24, Hq=1, Hk=1, D=256), dict(B=1 << 24, Hq=8, Hk=8, dtype=0), dict(B=1 << 23, Hq=1, Hk=1, D=256)):
+        assert attention(L, **kw) == UNSUPPORTED and b"workgroups" in L.yolo_last_error(), (kw, L.yolo_last_error())

@@ -590,6 +590,8 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
 // 804 us at one, 553 at two); one-wave workgroups run one to a SIMD, and f32 with more than 64 elements of o and q needs all 512 registers
 template <bool BF16, int DC, int WAVES, int CS = 1, int MW = (WAVES == 1 || (!BF16 && DC > 64)) ? 1 : 2>
 static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
+    const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk * CS;
+    YOLO_REQUIRE(launchable(blocks, WAVES * 64), YOLO_ERR_UNSUPPORTED, "cross_attention: %llu workgroups are more than one launch takes", blocks);
     constexpr int kLds = 2 * AttnTile<BF16, DC>::TILE + 2 * AttnTile<BF16, DC>::KT * AttnTile<BF16, DC / CS>::ROW;
     if (kLds > 64 * 1024) {
         static std::atomic<bool> attr_done[16];   // setting the attribute twice is harmless, the flag only must not tear
@@ -601,8 +603,6 @@ static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
             if (dev < 16) attr_done[dev] = true;
         }
     }
-    const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk * CS;
-    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 workgroups");
     hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
@@ -634,7 +634,7 @@ static int launch_attn(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
     }
     if (rc != YOLO_OK || p.splits == 1) return rc;
     const unsigned long long rows = (unsigned long long)p.B * p.Lq * p.Hq, blocks = p.splits > 8 ? rows : (rows * (p.D / 4) + 255) / 256;
-    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^31 rows");
+    YOLO_REQUIRE(launchable(blocks, 256), YOLO_ERR_UNSUPPORTED, "cross_attention: %llu workgroups are more than one launch takes", blocks);
     if (p.splits > 8) hipLaunchKernelGGL(cross_attention_join_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL(cross_attention_join_rows_kernel<BF16>, dim3((unsigned)blocks), dim3(256), 0, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
@@ -701,7 +701,7 @@ extern "C" int yolo_cross_attention(int dtype, const void* q, const int64_t* q_s
         return dtype == YOLO_DTYPE_BF16 ? launch_attn<true>(p, a, (hipStream_t)stream) : launch_attn<false>(p, a, (hipStream_t)stream);
     }
     const unsigned long long blocks = ((unsigned long long)B * Lq * Hq + 3) / 4;
-    YOLO_REQUIRE(blocks < (1ull << 31), YOLO_ERR_UNSUPPORTED, "cross_attention: more than 2^33 rows");
+    YOLO_REQUIRE(launchable(blocks, 256), YOLO_ERR_UNSUPPORTED, "cross_attention: %llu workgroups are more than one launch takes", blocks);
     if (dtype == YOLO_DTYPE_BF16) hipLaunchKernelGGL(cross_attention_general_kernel<true>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p);
     else hipLaunchKernelGGL(cross_attention_general_kernel<false>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, p);
     YOLO_HIP_CHECK(hipGetLastError());

@@ -48,6 +48,9 @@ __device__ __forceinline__ void dma16(const void* g, void* lds) {
                                      (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
+// The runtime counts the threads of a launch in 32 bits.
+static inline bool launchable(unsigned long long blocks, unsigned threads) { return blocks <= 0xffffffffull / threads; }
+
 static inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace yolo

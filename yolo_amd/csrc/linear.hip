@@ -466,7 +466,7 @@ template <bool BF16, int BM, int BN, int WR, int WC, bool ALIGNED>
 static int launch_tile(LinK k, hipStream_t stream) {
     constexpr int kLds = 2 * (BM + BN) * 128;
     const unsigned long long ntm = (k.M + BM - 1) / BM, ntn = (k.N + BN - 1) / BN;
-    YOLO_REQUIRE(ntm * ntn < (1ull << 31), YOLO_ERR_UNSUPPORTED, "linear: more than 2^31 tiles");
+    YOLO_REQUIRE(launchable(ntm * ntn, WR * WC * 64), YOLO_ERR_UNSUPPORTED, "linear: %llu tiles are more than one launch takes", ntm * ntn);
     k.ntm = (unsigned)ntm;
     k.ntn = (unsigned)ntn;
     if (kLds > 64 * 1024) {
@@ -487,7 +487,7 @@ static int launch_tile(LinK k, hipStream_t stream) {
 template <bool BF16, int TM, int TN, bool ALIGNED>
 static int launch_direct(LinK k, hipStream_t stream) {
     const unsigned long long ntm = (k.M + TM * 16 - 1) / (TM * 16), ntn = (k.N + TN * 16 - 1) / (TN * 16);
-    YOLO_REQUIRE(ntm * ntn < (1ull << 31), YOLO_ERR_UNSUPPORTED, "linear: more than 2^31 tiles");
+    YOLO_REQUIRE(launchable(ntm * ntn, 512), YOLO_ERR_UNSUPPORTED, "linear: %llu tiles are more than one launch takes", ntm * ntn);
     k.ntm = (unsigned)ntm;
     k.ntn = (unsigned)ntn;
     hipLaunchKernelGGL((linear_direct_kernel<BF16, TM, TN, ALIGNED>), dim3(k.ntm * k.ntn), dim3(512), 0, stream, k);

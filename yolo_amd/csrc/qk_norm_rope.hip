@@ -291,7 +291,7 @@ extern "C" int yolo_qk_norm_rope(int dtype, int B, int D, const void* q, const i
     }
     const unsigned long long total = blocks[0] + blocks[1];
     if (total == 0) return YOLO_OK;
-    YOLO_REQUIRE(total < (1ull << 31), YOLO_ERR_UNSUPPORTED, "qk_norm_rope: more than 2^31 workgroups");
+    YOLO_REQUIRE(launchable(total, 256), YOLO_ERR_UNSUPPORTED, "qk_norm_rope: %llu workgroups are more than one launch takes", total);
     p.blocks0 = (unsigned)blocks[0];
     if (dtype == YOLO_DTYPE_BF16) launch_rope<true>(p, lpr, (unsigned)total, (hipStream_t)stream);
     else launch_rope<false>(p, lpr, (unsigned)total, (hipStream_t)stream);
