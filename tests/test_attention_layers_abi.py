@@ -86,3 +86,12 @@ def test_launches_past_the_runtime_limit_are_refused(L):
     for kw in (dict(B=1 << 10, Lq=1 << 13, Hq=8, Hk=8, Lk=0), dict(B=1 << 10, Lq=1 << 13, Hq=8, Hk=8, D=7), dict(B=1 << 26, Hq=1, Hk=1),
                dict(B=1 << 24, Hq=1, Hk=1, D=128), dict(B=1 << 24, Hq=1, Hk=1, D=256), dict(B=1 << 24, Hq=8, Hk=8, dtype=0), dict(B=1 << 23, Hq=1, Hk=1, D=256)):
         assert attention(L, **kw) == UNSUPPORTED and b"workgroups" in L.yolo_last_error(), (kw, L.yolo_last_error())
+
+
+def test_no_row_kernel_that_no_call_reaches(L):
+    """A row of at most 256 elements is 32 pairs of 16-byte pieces in float32 and 16 in bfloat16: the library has no bfloat16 kernel of 32 lanes."""
+    from yolo_amd import _lib
+    with open(_lib.LIB_PATH, "rb") as f:
+        built = f.read()
+    assert b"qk_norm_rope_kernelILb0ELi32E" in built and b"qk_norm_rope_kernelILb1ELi16E" in built
+    assert b"qk_norm_rope_kernelILb1ELi32E" not in built

@@ -226,7 +226,12 @@ static void launch_rope(const RopeK& p, int lpr, unsigned blocks, hipStream_t st
         case 4: launch_rope_rows<BF16, 4>(p, blocks, stream); break;
         case 8: launch_rope_rows<BF16, 8>(p, blocks, stream); break;
         case 16: launch_rope_rows<BF16, 16>(p, blocks, stream); break;
-        case 32: launch_rope_rows<BF16, 32>(p, blocks, stream); break;
+        case 32:
+            if constexpr (!BF16) {                              // a bf16 row is at most 16 pairs of pieces
+                launch_rope_rows<BF16, 32>(p, blocks, stream);
+                break;
+            }
+            [[fallthrough]];
         default: hipLaunchKernelGGL(qk_norm_rope_general_kernel<BF16>, dim3(blocks), dim3(256), 0, stream, p);
     }
 }
