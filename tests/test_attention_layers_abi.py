@@ -95,3 +95,14 @@ def test_no_row_kernel_that_no_call_reaches(L):
         built = f.read()
     assert b"qk_norm_rope_kernelILb0ELi32E" in built and b"qk_norm_rope_kernelILb1ELi16E" in built
     assert b"qk_norm_rope_kernelILb1ELi32E" not in built
+
+
+def test_objects_depend_on_the_makefile():
+    """A changed flag (such as the one against packed float32 arithmetic) compiles every source again."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "yolo_amd", "csrc")
+    plan = subprocess.run(["make", "-n", "-W", "Makefile"], cwd=csrc, check=True, capture_output=True, text=True).stdout
+    for f in sorted(os.listdir(csrc)):
+        if f.endswith(".hip"):
+            assert "-c " + f in plan, f
