@@ -151,6 +151,16 @@ _ACTIVATIONS = {None: 0, "linear": 0, "leaky": 1, "relu": 2, "gelu": 3, "silu": 
 
 
 _Strides = ctypes.c_int64 * 3
+_BF16 = torch.bfloat16
+_INT_MAX = 0x7fffffff
+
+
+def _no_tangents(**operands):
+    """Forward-mode dual tensors would come out without their tangents.  Called inside a level of forward_ad only: looking at an operand
+    costs 0.3 us."""
+    for name, x in operands.items():
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            raise ValueError("%s has a tangent: yolo_amd implements the inference path only (no forward-mode derivatives)" % name)
 
 
 def _dev(x, name, dev, dtype=None):
@@ -161,9 +171,7 @@ def _dev(x, name, dev, dtype=None):
             x = x.float()
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("%s requires a gradient: yolo_amd implements the inference path only (call under torch.no_grad())" % name)
-    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(x).tangent is not None:       # unpack_dual alone costs 0.3 us outside a level
-        raise ValueError("%s has a tangent: yolo_amd implements the inference path only (no forward-mode derivatives)" % name)
-    if x.is_neg():                                                    # imaginary part of a conjugate: memory holds the negatives
+    if x.dtype is not _BF16 and x.is_neg():                           # imaginary part of a conjugate: memory holds the negatives
         x = x.resolve_neg()
     if dtype is not None and x.dtype != dtype:
         x = x.to(dtype)
@@ -196,8 +204,8 @@ def _param(x, n, name, dev):
 
 
 def _fits(name, *sizes):
-    """The C entries take int sizes, and ctypes would pass on the low 32 bits of a longer one."""
-    if max(sizes) > 0x7fffffff:
+    """The C entries take int sizes, and ctypes would pass on the low 32 bits of a longer one.  Called for tensors of 2^31 elements and more."""
+    if max(sizes) > _INT_MAX:
         raise ValueError("%s: sizes %s, each must be below 2^31" % (name, sizes))
 
 
@@ -236,6 +244,8 @@ def linear(inputs, weight, bias=None, activation=None, residual=None):
     """act(inputs @ weight.T + bias) + residual in one launch: inputs [..., K] (a map's cells [B, H, W, K] as they are), weight
     [N, K], bias [N], residual [..., N] -> [..., N], float32 or bfloat16 throughout (bias: either).  activation: None, "leaky"
     (slope 0.1), "relu", "gelu" (error function) or "silu"; the residual is added after it, as in res_block.  yolo_linear."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(inputs=inputs, weight=weight, bias=bias, residual=residual)
     dev = _gpu()
     x, w = _dev(inputs, "inputs", dev), _dev(weight, "weight", dev)
     code = _code(x, "inputs")
@@ -247,7 +257,8 @@ def linear(inputs, weight, bias=None, activation=None, residual=None):
     if not shape or len(wshape) != 2 or wshape[1] != shape[-1] or wshape[1] == 0 or wshape[0] == 0:
         raise ValueError("linear: inputs %s do not fit weight %s" % (shape, tuple(wshape)))
     N, K = wshape
-    _fits("linear", N, K)
+    if w.numel() > _INT_MAX:
+        _fits("linear", N, K)
     b, bcode = _param(bias, N, "bias", dev)
     shape = shape[:-1] + (N,)
     r, r_ld = None, 0
@@ -278,7 +289,8 @@ def _heads(x, name):
     """[B, L, H, D] with a contiguous last dimension -> (tensor, ctypes strides of batch, token, head)."""
     if x.dim() != 4:
         raise ValueError("%s must be [B, L, H, D], got %s" % (name, tuple(x.shape)))
-    _fits(name, *x.shape)
+    if x.numel() > _INT_MAX:
+        _fits(name, *x.shape)
     st = x.stride()
     if st[3] != 1 and x.shape[3] > 1:
         x = x.contiguous()
@@ -296,9 +308,8 @@ def _attention_operand(x, D):
     return x, _Strides(st[0], st[1], st[2])
 
 
-def _positions(p, B, L, axes, name, dev):
-    """-> (contiguous tensor, batched).  [L] / [B, L] for one axis, [L, 2] / [B, L, 2] for two; a trailing 1 is allowed for one."""
-    p = _dev(p, name, dev)
+def _positions(p, B, L, axes, name):
+    """Tensor on the GPU -> (contiguous tensor, batched).  [L] / [B, L] for one axis, [L, 2] / [B, L, 2] for two; a trailing 1 is allowed for one."""
     if p.dtype not in (torch.int32, torch.int64):
         raise ValueError("%s must be int32 or int64, got %s" % (name, p.dtype))
     shape = tuple(p.shape)
@@ -319,6 +330,8 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, frequencies=None, q_positio
     column), where the first half of the pairs turns by the row and the second by the column.  `axes` (1 or 2) says which where
     None would leave [B, L] = [L, 2] open.  Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) if `interleaved`.
     yolo_qk_norm_rope."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(q=q, k=k, q_weight=q_weight, k_weight=k_weight, frequencies=frequencies)
     dev = _gpu()
     q, qs = _heads(_dev(q, "q", dev), "q")
     code = _code(q, "q")
@@ -350,9 +363,9 @@ def qk_norm_rope(q, k, q_weight=None, k_weight=None, frequencies=None, q_positio
             axes = 2 if q_positions.dim() > 1 and q_positions.shape[-1] == 2 and tuple(q_positions.shape) != (B, Lq) else 1
         if axes not in (1, 2) or R // 2 % axes:
             raise ValueError("qk_norm_rope: %d pairs over %r axes" % (R // 2, axes))
-        qp, qb = _positions(q_positions, B, Lq, axes, "q_positions", dev)
+        qp, qb = _positions(q_positions, B, Lq, axes, "q_positions")
         if k is not None:
-            kp, kb = _positions(k_positions, B, Lk, axes, "k_positions", dev)
+            kp, kb = _positions(_dev(k_positions, "k_positions", dev), B, Lk, axes, "k_positions")
             if kp.dtype != qp.dtype:
                 kp, qp = kp.long(), qp.long()
         pos64 = int(qp.dtype == torch.int64)
@@ -378,6 +391,8 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.  D up to 256;
     tensors whose rows do not start on 16 bytes are copied first, head sizes that are not multiples of 8 padded.
     -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
+    if forward_ad._current_level >= 0:
+        _no_tangents(q=q, k=k, v=v)
     dev = _gpu()
     q = _dev(q, "q", dev)
     code = _code(q, "q")
@@ -386,7 +401,8 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
         raise ValueError("cross_attention: q %s and k %s must be [B, L, H, D]" % (tuple(q.shape), tuple(k.shape)))
     B, Lq, Hq, D = q.shape
     Lk, Hk = k.shape[1:3]
-    _fits("cross_attention", B, Lq, Lk, Hq, Hk, D)
+    if q.numel() > _INT_MAX or k.numel() > _INT_MAX:
+        _fits("cross_attention", B, Lq, Lk, Hq, Hk, D)
     if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
         raise ValueError("cross_attention: q %s, k %s, v %s do not fit" % (tuple(q.shape), tuple(k.shape), tuple(v.shape)))
     if D == 0 or Hk == 0 or Hq == 0 or Hq % Hk:
