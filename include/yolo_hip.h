@@ -232,8 +232,10 @@ int yolo2_nms(const double* boxes, const float* probs, int B, int n, int C, floa
 
 /* ---- attention-side layers (no counterpart in the reference): what a head needs in which cells, queries or prompts attend to
  * the maps of the networks above.  Inference only.  Element type float32 or bfloat16 (`dtype`: YOLO_DTYPE_*) for every
- * activation and weight matrix; arithmetic, sums and softmax in float32, one rounding at the store (cross_attention in bfloat16 also
- * rounds the weights of the values).  Outputs must not overlap inputs; memory the outputs do not name is left as it was.  None
+ * activation and weight matrix; arithmetic, sums and softmax in float32, one rounding at the store.  Two exceptions in bfloat16:
+ * cross_attention rounds the weights of the values to bfloat16 where a key head serves more than 32 rows (queries times the query heads
+ * that share it; of fewer it keeps them to 2^-15), and gelu and silu of linear are within 2^-14 of their value before the rounding
+ * (silu below 10^-36 may be 0).  Outputs must not overlap inputs; memory the outputs do not name is left as it was.  None
  * allocates, synchronises or keeps anything between calls, so calls may overlap on any streams (each with a workspace of its
  * own) and may be captured into a HIP graph.  A call repeated gives the same bits; the kernel and the order of its sums go by the
  * sizes of the call, so a row may differ in its last bits between calls of other batch sizes.  Sizes that need 2^32 threads or more in a

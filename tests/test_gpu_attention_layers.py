@@ -780,3 +780,22 @@ def test_gelu_is_relatively_exact_in_the_negative_tail(L, t, n):
     bound = (u * (1 + formula) + formula + v64 * v64 * 2.0 ** -22) * y.abs() + 1e-38
     got = L.linear(x, w, activation="gelu")
     within(got, y[:, None].expand(-1, n), bound[:, None].expand(-1, n), (t, n))
+
+
+@pytest.mark.parametrize("b,lq,lk,hq,hk,d", [(1, 1, 3549, 16, 4, 64), (2, 3, 200, 8, 2, 128), (3, 8, 300, 4, 1, 32), (1, 32, 150, 2, 2, 96), (1, 5, 400, 2, 1, 256),
+                                             (300, 1, 200, 16, 4, 64), (600, 2, 130, 4, 2, 32), (1, 1, 900, 4, 4, 200)])
+def test_attention_of_few_queries_keeps_whole_weights(L, b, lq, lk, hq, hk, d):
+    """bfloat16 with up to 32 rows a head group: the weights are the upper 16 bits and the rest rounded to bfloat16.  Cutting leaves less than 2^-7
+    of a weight, and rounding that is off by 2^-8 of it: 2^-15 of a weight where one rounding to bfloat16 is 2^-8."""
+    q, k, v = qkv(BF16, b, lq, lk, hq, hk, d, 300)
+    got = L.cross_attention(q, k, v)
+    g, u = hq // hk, torch.finfo(BF16).eps / 2
+    q64, k64, v64 = (x.double().cpu() for x in (q, k, v))
+    for i in range(0, b, max(1, b // 20)):
+        for h in range(hq):
+            qq, kk, vv = q64[i, :, h], k64[i, :, h // g], v64[i, :, h // g]
+            ds = float((qq.abs() @ kk.abs().t()).max()) * d ** -0.5 * (d + 4) * 2.0 ** -24
+            p = torch.softmax(qq @ kk.t() * d ** -0.5, -1)
+            ref = p @ vv
+            bound = (np.expm1(2 * ds) + 2 * lk * 2.0 ** -24 + 2.0 ** -18 + 2.0 ** -15) * 2 * (p @ vv.abs())
+            within(got[i, :, h], ref, bound * (1 + u) + u * ref.abs(), (b, lq, lk, hq, hk, d, i, h))

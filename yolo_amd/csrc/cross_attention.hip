@@ -122,7 +122,11 @@ __global__ __launch_bounds__(256) void cross_attention_general_kernel(AttnK p) {
 // The running maximum is only raised when a score exceeds it by 2^8 in weight: weights stay below 2^8, which costs no precision
 // (they are floating point) and most tiles skip the rescaling of o.
 // bf16: the weights are rounded to bf16 for the second product, at most 2^-8 of each and of either sign, which is the size of the
-// rounding of the result; their sum is taken of the f32 values.
+// rounding of the result; their sum is taken of the f32 values.  The error of a result against float64 is 0.0023 of its size with that, 0.0017
+// without.  Where a head group has no more than 32 rows (WHOLE) the weights go in as two bf16, the upper 16 bits and the rest, within 2^-15
+// of themselves, and both are multiplied: such calls wait for k and v (one query of 16 / 4 heads of 64 over 3549 keys 10.0 against 9.4 us,
+// 64 of them 50.0 against 49.8).  With more rows the products bound the call and a third half as much again shows: 8 x 676 over 2704 keys, 8 heads
+// of 64, 77 against 58 us, 8 x 2704 over 5776 of 128 718 against 548.
 //
 // CS > 1: the columns of v and of the result are divided over CS workgroups, each of which forms all the scores.  At D = 256 that halves
 // the registers of o: two workgroups of a CU instead of one hide each other's latencies in bf16, 4 x 1000 x 2000 keys of 4 heads 70 us
@@ -149,7 +153,7 @@ template <bool BF16, int DC> struct AttnTile {
     }
 };
 
-template <bool BF16, int DC, int WAVES, int MW, int CS>
+template <bool BF16, int DC, int WAVES, int MW, int CS, bool WHOLE>
 __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(AttnK p) {
     typedef typename Elem<BF16>::type T;
     typedef AttnTile<BF16, DC> L;                           // k
@@ -348,11 +352,19 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
             if constexpr (BF16) {
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {               // 16 keys: registers 8 g .. 8 g + 7
-                    bf16x8 fp;
-                    u32x4 pk;
+                    u32x4 pk, rest;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) pk[j] = pack_bf16(s[kb][8 * g + 2 * j], s[kb][8 * g + 2 * j + 1]);
-                    fp = __builtin_bit_cast(bf16x8, pk);
+                    for (int j = 0; j < 4; ++j) {
+                        const float w0 = s[kb][8 * g + 2 * j], w1 = s[kb][8 * g + 2 * j + 1];
+                        if constexpr (WHOLE) {
+                            const uint32_t b0 = __float_as_uint(w0), b1 = __float_as_uint(w1);
+                            pk[j] = b0 >> 16 | (b1 & 0xffff0000u);
+                            rest[j] = pack_bf16(w0 - __uint_as_float(b0 & 0xffff0000u), w1 - __uint_as_float(b1 & 0xffff0000u));
+                        } else {
+                            pk[j] = pack_bf16(w0, w1);
+                        }
+                    }
+                    const bf16x8 fp = __builtin_bit_cast(bf16x8, pk);
                     // lane's address for the transposed read: key row (lane / 4) % 4 of its four keys, 4 elements at 4 (lane % 4)
                     const int key = kb * 32 + 16 * g + 4 * half + ((lane >> 2) & 3);
 #pragma unroll
@@ -366,6 +378,7 @@ __global__ __launch_bounds__(WAVES * 64, MW) void cross_attention_tile_kernel(At
                         typedef short s16x8 __attribute__((ext_vector_type(8)));
                         const bf16x8 fv = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
                         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv, fp, o[i], 0, 0, 0);
+                        if constexpr (WHOLE) o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv, __builtin_bit_cast(bf16x8, rest), o[i], 0, 0, 0);
                     }
                 }
             } else {
@@ -517,6 +530,7 @@ __global__ __launch_bounds__(256) void cross_attention_join_rows_kernel(AttnK p)
 // ---- plan: the tile shape and the number of key splits, by sizes and type alone ---------------------------------------------------
 struct AttnPlan {
     int dc, waves, kt, rtiles, cs, splits, tps;     // cs: column parts of v
+    bool few;                                       // no more than 32 rows of a head group
     size_t bytes;
 };
 
@@ -526,7 +540,7 @@ struct AttnPlan {
 // heads of 64, 4 key heads: 9.1 at S = 1, 8.5 at 5 over 300 keys; 28 at 1, 8.9 at 12 over 1444; 64 at 1, 10 at 28 over 3549.
 // Eight waves share a tile's loads where their larger row tiles still fill the CUs as well (8 x 2704 queries of 8 heads of 128: 524
 // against 553), not over few tiles (80 keys, above: 153).
-// Up to 32 rows of a head group need one wave, but four load a tile faster while CUs are free (one query of 16 / 4 heads of 64 over 3549 keys
+// Up to 32 rows of a head group (measured with weights of one bf16, which take 0.6 to 0.8 us less) need one wave, but four load a tile faster while CUs are free (one query of 16 / 4 heads of 64 over 3549 keys
 // 9.4 against 10.3 us, 2 of 2 heads of 96 over 217: 8.4 against 13.2), and at 96 and more in bf16 as many workgroups of four waves fit a CU as of one;
 // one-wave workgroups where they fill the CUs several times (16 x that query 19 against 23, f32 54 against 72).
 static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int D) {
@@ -537,7 +551,7 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
     const long long rows = (long long)Lq * (Hq / Hk), groups = (long long)B * Hk;
     auto rtiles = [&](int waves) { return (rows + 32 * waves - 1) / (32 * waves); };
     auto rounds = [](long long blocks, long long slots) { return (blocks + slots - 1) / slots; };
-    const bool few = rows <= 32;
+    const bool few = a.few = rows <= 32;
     const int tiles = (Lk + a.kt - 1) / a.kt;
     int wide = 4;                                           // waves of a workgroup where there are rows for more than one
     if (bf16 && a.dc >= 64 && a.dc <= 128 && tiles >= 8 && rtiles(8) * groups >= 512 && rounds(rtiles(8) * groups, 256) <= rounds(rtiles(4) * groups, 512)) wide = 8;
@@ -588,8 +602,9 @@ static AttnPlan attn_plan(int dtype, int B, int Lq, int Lk, int Hq, int Hk, int 
 
 // MW: waves per SIMD the register budget is cut for.  Two hide each other's latencies where the tiles fill the GPU (D = 128, four waves:
 // 804 us at one, 553 at two); one-wave workgroups run one to a SIMD, and f32 with more than 64 elements of o and q needs all 512 registers
-template <bool BF16, int DC, int WAVES, int CS = 1, int MW = (WAVES == 1 || (!BF16 && DC > 64)) ? 1 : 2>
+template <bool BF16, int DC, int WAVES, int CS, bool WHOLE>
 static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
+    constexpr int MW = (WAVES == 1 || (!BF16 && DC > 64)) ? 1 : 2;
     const unsigned long long blocks = (unsigned long long)p.rtiles * p.splits * p.B * p.Hk * CS;
     YOLO_REQUIRE(launchable(blocks, WAVES * 64), YOLO_ERR_UNSUPPORTED, "cross_attention: %llu workgroups are more than one launch takes", blocks);
     constexpr int kLds = 2 * AttnTile<BF16, DC>::TILE + 2 * AttnTile<BF16, DC>::KT * AttnTile<BF16, DC / CS>::ROW;
@@ -598,28 +613,38 @@ static int launch_attn_tile(const AttnK& p, hipStream_t stream) {
         int dev = 0;
         YOLO_HIP_CHECK(hipGetDevice(&dev));
         if (dev >= 16 || !attr_done[dev]) {
-            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS>,
+            YOLO_HIP_CHECK(hipFuncSetAttribute((const void*)cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS, WHOLE>,
                                                hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
             if (dev < 16) attr_done[dev] = true;
         }
     }
-    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
+    hipLaunchKernelGGL((cross_attention_tile_kernel<BF16, DC, WAVES, MW, CS, WHOLE>), dim3((unsigned)blocks), dim3(WAVES * 64), kLds, stream, p);
     YOLO_HIP_CHECK(hipGetLastError());
     return YOLO_OK;
 }
 
+// bf16 with few rows: whole weights, one or four waves
 template <bool BF16, int DC>
 static int launch_attn_dc(const AttnK& p, const AttnPlan& a, hipStream_t stream) {
-    if constexpr (BF16 && (DC == 64 || DC == 96 || DC == 128)) {
-        if (a.waves == 8) return launch_attn_tile<BF16, DC, 8>(p, stream);
+    constexpr int CS = BF16 && DC == 256 ? 2 : 1;
+    if constexpr (BF16) {
+        if (a.few) {
+            if constexpr (DC <= 64) {
+                if (a.waves == 1) return launch_attn_tile<BF16, DC, 1, 1, true>(p, stream);
+            }
+            return launch_attn_tile<BF16, DC, 4, CS, true>(p, stream);
+        }
+        if constexpr (DC == 64 || DC == 96 || DC == 128) {
+            if (a.waves == 8) return launch_attn_tile<BF16, DC, 8, 1, false>(p, stream);
+        }
+    } else {
+        if constexpr (DC < 256) {
+            if (a.waves == 1) return launch_attn_tile<BF16, DC, 1, 1, false>(p, stream);
+        } else {
+            if (a.cs == 2) return launch_attn_tile<BF16, DC, 4, 2, false>(p, stream);
+        }
     }
-    if constexpr (DC <= 64 || (!BF16 && DC < 256)) {
-        if (a.waves == 1) return launch_attn_tile<BF16, DC, 1>(p, stream);
-    }
-    if constexpr (DC == 256) {
-        if (BF16 || a.cs == 2) return launch_attn_tile<BF16, DC, 4, 2>(p, stream);
-    }
-    if constexpr (!BF16 || DC < 256) return launch_attn_tile<BF16, DC, 4>(p, stream);
+    return launch_attn_tile<BF16, DC, 4, CS, false>(p, stream);
 }
 
 template <bool BF16>

@@ -388,7 +388,8 @@ def cross_attention(q, k, v, key_lens=None, key_mask=None, scale=None):
     """softmax(scale * q k^T) v: q [B, Lq, Hq, D] over the states k, v [B, Lk, Hk, D] of another length (any strides over a
     contiguous D, so the halves of one key / value projection go in as views); Hq a multiple of Hk, query head h reads key head
     h // (Hq // Hk).  key_lens [B] int32: keys from key_lens[b] on are padding; key_mask [B, Lk] bool: False leaves a key out.
-    What is left out has no influence whatever it holds; a row with no key left is zero.  scale: None = D ** -0.5.  D up to 256;
+    What is left out has no influence whatever it holds; a row with no key left is zero. bfloat16 rounds the weights of the
+    values where a key head serves more than 32 rows (queries times the query heads that share it).  scale: None = D ** -0.5.  D up to 256;
     tensors whose rows do not start on 16 bytes are copied first, head sizes that are not multiples of 8 padded.
     -> [B, Lq, Hq, D] packed.  yolo_cross_attention."""
     if forward_ad._current_level >= 0:
