@@ -129,11 +129,11 @@ __device__ __forceinline__ u32x4 place_piece(u32x4 v, int k, int K) {
 // ALIGNED: rows of x and W start on 16 bytes and K is whole pieces; they go global -> LDS by DMA, pieces past K from a zero piece.
 // Otherwise the pieces pass through registers.
 //
-// Measured, bf16: 8192^3 1.31 PFLOP/s with 256 x 256 tiles of 16 waves (64 x 64 each, 116 registers, one workgroup a CU), 1.11 with
-// 128 x 128 (two a CU); the library's product reaches 1.08 on the same card.  23104 x 4096 x 1024 with gelu 0.87 PFLOP/s: six rounds of
-// 256 tiles, between which loads, stores and the activation are not covered by products.  173056 x 512 x 256 with gelu and residual
-// 3.3 TB/s, bandwidth and the same gaps.  Persistent workgroups that fetch the next tile before the epilogue were slower (128
-// registers do not hold both); f32 117 TFLOP/s at 23104 x 1024 x 512 (the f32 matrix peak is 157).
+// Measured, bf16: 8192^3 1.36 PFLOP/s with 256 x 256 tiles of 16 waves (64 x 64 each, 116 registers, one workgroup a CU), a fifth less with
+// 128 x 128 (two a CU); the library's product reaches 1.65 on the same card.  23104 x 4096 x 1024 1.07 PFLOP/s, as the library, and with gelu
+// 0.88: six rounds of 256 tiles, between which loads, stores and the activation are not covered by products.  173056 x 512 x 256 with gelu
+// and residual 3.3 TB/s, bandwidth and the same gaps.  Persistent workgroups that fetch the next tile before the epilogue were slower (128
+// registers do not hold both); f32 115 to 120 TFLOP/s at 23104 x 1024 x 512 (the library 100; 154 at 8192^3).
 __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};
 
 // Swaps lane rows so that a lane that holds 4 outputs of each of two 16-wide tiles (a: tile i, b: tile i + 1, packed pairs) holds 8
@@ -496,7 +496,7 @@ static int launch_direct(LinK k, hipStream_t stream) {
 }
 
 // Tile by the time that the rounds of its tiles on the 256 CUs take.
-// bf16, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU takes 4 (1309 TFLOP/s at 8192^3, 128 x 128 1105 with twice the
+// bf16, in units of a 128 x 128 tile's share of a CU: one 256 x 256 tile a CU takes 4 (1.3 PFLOP/s at 8192^3, 128 x 128 1.1 with twice the
 // operand traffic), two of 192 x 128 3.35, two of 128 x 128 2.55, four of 64 x 64 1.75: fitted to 67 shapes (600 to 200000 rows, 48 to 8192
 // wide), where the choice is 2 % from the best of six tiles on average.  Measured (us for 256 / 192 / 128 / 64): 23104 x 4096 x 1024 217 / 227 /
 // 244 / 319, 5000 x 2048 x 2048 55 / 45 / 58 / 69, 8000 x 1024 x 1024 30 / 26 / 23 / 34, 2704 x 1024 x 256 15.5 / 9.4 / 8.8 / 6.9.
@@ -521,7 +521,7 @@ static int launch_linear(const LinK& k, bool aligned, hipStream_t stream) {
         const unsigned long long n = (unsigned long long)((k.M + bm - 1) / bm) * ((k.N + bn - 1) / bn);
         return (double)((n + slots - 1) / slots);
     };
-    // where pieces pass through registers, sixteen waves of 32 x 32 take 100 us against 103 with four of 64 x 64 at 23104 x 1024 x 1023, and
+    // where pieces pass through registers (operands out of HBM), sixteen waves of 32 x 32 take 100 us against 103 with four of 64 x 64 at 23104 x 1024 x 1023, and
     // eight of 16 x 32 7.1 against 8.1 with four of 32 x 32 at 1001 x 255 x 255; in f32 likewise 207 against 215 at 23104 x 1024 x 512 and 35 against 37
     // at 5408 x 512 x 512
     if constexpr (BF16) {
